@@ -94,7 +94,7 @@ def prepare(case, seed):
         if case["delta"] != "none":
             s["delta"] = randn(rows, k).to(torch.bfloat16 if case["delta"] == "bf16" else torch.float32)
         s["w"] = randn(k).mul_(0.1)
-        s["eps"] = 1e-6
+        s["eps"] = 2.0 ** -20   # a single-precision number, so that every form adds the same one
         s["q"] = torch.empty(rows, k, dtype=torch.int8, device="cuda")
         s["scale"] = torch.empty(rows, device="cuda")
         s["sum"] = torch.empty(rows, k, device="cuda") if s["delta"] is not None else None
