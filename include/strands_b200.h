@@ -60,16 +60,25 @@ int b200_read_fault(unsigned int* fault_out);
  *                   of the logical tensor each row belongs to)
  *   B200_W_TERNARY  data uint8 [n, k/4] (2 bits per element: 00=0, 01=+1, 11=-1),
  *                   scales bf16 [n]
+ *   B200_W_INT8     data int8 [n, k], row_scale fp32 [n] (element = code x row scale). Not
+ *                   weight-only: read by b200_linear_int8, whose activations are int8 too; the
+ *                   entry points that stream or dequantise weights refuse it.
  */
-enum b200_wfmt { B200_W_BF16 = 0, B200_W_INT4G128 = 1, B200_W_NVFP4 = 2, B200_W_TERNARY = 3 };
+enum b200_wfmt {
+  B200_W_BF16 = 0,
+  B200_W_INT4G128 = 1,
+  B200_W_NVFP4 = 2,
+  B200_W_TERNARY = 3,
+  B200_W_INT8 = 4
+};
 
 typedef struct b200_qweight {
   int32_t format;
   int32_t n; /* rows (output features), a multiple of 256 for b200_linear */
-  int32_t k; /* columns (input features), a multiple of 128 */
+  int32_t k; /* columns (input features), a multiple of 128 (INT8: of 16) */
   const void* data;
   const void* scales;
-  const float* row_scale; /* NVFP4 only, else NULL */
+  const float* row_scale; /* NVFP4 and INT8, else NULL */
   /* The GEMM's streaming copy of data/scales (b200_tile_weights): one contiguous chunk per
    * (256-row tile, 64-column stage), so each stage is one bulk copy. Required by
    * b200_linear for the packed formats; NULL for bf16 (read through a tensor map). */
@@ -78,7 +87,8 @@ typedef struct b200_qweight {
 } b200_qweight;
 
 /* Quantise an fp32 weight w[n, k] (one logical nn.Linear) into `format`; writes data,
- * scales and (NVFP4) row_scale[n]. Bit-exact to oracle/quant.py. */
+ * scales (not INT8) and (NVFP4, INT8) row_scale[n]. Bit-exact to oracle/quant.py. INT8 takes the
+ * rows as b200_quantize_act_int8 does: w and data 16-byte aligned, k a multiple of 16, <= 65536. */
 int b200_quantize(int32_t format, const float* w, int32_t n, int32_t k, void* data, void* scales,
                   float* row_scale, b200_stream stream);
 /* Unpack a packed weight to bf16 out[n, k], exactly as the GEMM's shared-memory unpacker. */
@@ -168,6 +178,50 @@ int b200_nvfp4_sf_atoms(const uint8_t* scales, int32_t rows, int32_t k, uint8_t*
  * n_valid rules as b200_linear (SwiGLU writes bf16 planes). */
 int b200_linear_nvfp4_native(const uint8_t* x_codes, const uint8_t* x_sf, int32_t m, int32_t k, const b200_qweight* w,
                              const uint8_t* w_sf, const b200_linear_out* out, b200_stream stream);
+
+/* ---------------------------------------------------------------- 8-bit integer linears (W8A8)
+ * Activations and weights as int8 codes with one fp32 scale per token and one per output channel:
+ *   y[t, n] = (sum_k q[t, k] * w[n, k]) * scale[t] * row_scale[n],
+ * the sum exact in int32. Replaces the same `nn.Linear` calls as b200_linear (TF:417-420,
+ * TF:632-643, TF:701-703) at twice the bf16 tensor rate and in one pass, at about 7 significant
+ * bits per activation row: for callers that accept W8A8 (a model of B200_W_INT8 weights runs on
+ * it, see b200_model_create).
+ *
+ * Codes of a row v[0..k) (fp32; fl = one fp32 rounding, rint = half to even):
+ *   a = max |v|, scale = fl(a / 127), q[i] = rint(fl(v[i] * fl(127 / a))), in [-127, 127];
+ *   a row whose scale is below 2^-126 (all zeros, or nothing a normal number can scale): scale 0
+ *   and codes 0; a row with an infinity or NaN: scale NaN and codes 0, so that every product of
+ *   that row is NaN and no other row is touched. */
+enum b200_act_type { B200_ACT_F32 = 0, B200_ACT_BF16 = 1 };
+
+/* Int8 codes q [rows, ldq] and scales [rows] of x [rows, ldx] (fp32, or bf16 bit patterns). With
+ * x_lo (bf16 only, same ldx) the row is v = fl(x + x_lo): the two planes the mixers and the SwiGLU
+ * epilogue write. k a multiple of 16, at most 65536; ldx in elements, ldx * element size and ldq
+ * multiples of 16; x, x_lo and q 16-byte aligned. Columns k .. ldq - 1 of q are left as they
+ * were. */
+int b200_quantize_act_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t rows, int32_t k, int32_t ldx,
+                           int8_t* q, int32_t ldq, float* scale, b200_stream stream);
+
+/* The residual addition, Qwen3_5RMSNorm (TF:711-728) and the codes in one pass:
+ *   t = fl(x + delta); r = fl((S / hidden + eps)^-1/2), S = sum t^2 in 64 bits;
+ *   v = fl(fl(t * r) * fl(1 + w)); q, scale = the codes of v.
+ * x fp32 [rows, ldx]; delta (optional) fp32 or bf16 [rows, ldd]; sum (optional, needs delta)
+ * receives t as fp32 [rows, lds] and may be x or an fp32 delta themselves (same stride), with no
+ * other overlap. hidden a multiple of 16, at most 65536; every row stride in bytes a multiple of
+ * 16 and every pointer 16-byte aligned; eps >= 0. */
+int b200_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd, float* sum,
+                      int32_t lds, int32_t rows, int32_t hidden, const float* w, float eps, int8_t* q, int32_t ldq,
+                      float* scale, b200_stream stream);
+
+/* The product above with b200_linear's epilogues, for q [m, ldx] codes (any int8 values, from
+ * either call above or the caller's own), x_scale [m] and a B200_W_INT8 weight. Any m >= 1 and any
+ * w->n; k = w->k a multiple of 16, at most 65536; ldx a multiple of 16; q and w->data 16-byte
+ * aligned. Only columns < n_valid are written: any n_valid <= w->n for STORE and RESID_ADD; a
+ * multiple of 128 for SWIGLU, whose weight rows are interleaved in blocks of 64 (gate, up). The
+ * SwiGLU's lo plane follows lo_offset and lo_format as in b200_linear. ldo: any that holds a row.
+ * Results do not depend on the batch a row is in, nor on timing. */
+int b200_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
+                     const b200_linear_out* out, b200_stream stream);
 
 /* ---------------------------------------------------------------- ragged batches, prefix cache */
 typedef struct b200_seqs {

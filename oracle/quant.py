@@ -37,6 +37,13 @@ Ternary (BitNet b1.58 absmean, Ma et al. 2024), per-output-row scale
                   00 = 0, 01 = +1, 11 = -1
     dequant     bf16_rn(t * float(scale[n]))  (exact)
 
+Int8 rows (weights per output channel, activations per token: the W8A8 linears)
+    a           = amax(|v|) of the row v (for two-plane activations v = fp32(hi + lo))
+    scale       = fp32(a / 127); below 2^-126: scale 0 and codes 0; a row with an infinity
+                  or NaN: scale NaN and codes 0
+    code        = rint_half_even(fp32(v * fp32(127 / a))), in [-127, 127]
+    dequant     float(code) * scale (fp32)
+
 bf16_rn is IEEE round-to-nearest-even of an fp32 value to bfloat16.
 """
 
@@ -356,9 +363,45 @@ def dequantize_ternary(packed: np.ndarray, sbits: np.ndarray) -> np.ndarray:
     return (t * s[:, None]).astype(np.float32)
 
 
+# ----------------------------------------------------------------------------- int8 rows
+
+
+def quantize_int8_rows(v: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """fp32 [rows, K] -> (codes int8 [rows, K], scales fp32 [rows]), every step one fp32
+    rounding (numpy's fp32 quotients and products are)."""
+    v = np.ascontiguousarray(v, dtype=np.float32)
+    finite = np.isfinite(v).all(axis=1)
+    with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
+        a = np.abs(v).max(axis=1)
+        scale = (a / np.float32(127.0)).astype(np.float32)
+        live = finite & (scale >= np.float32(2.0 ** -126))
+        inv = np.where(live, np.float32(127.0) / a, np.float32(0)).astype(np.float32)
+        prod = np.where(live[:, None], v, np.float32(0)) * inv[:, None]
+    codes = np.rint(prod.astype(np.float32)).astype(np.int8)
+    return codes, np.where(finite, np.where(live, scale, np.float32(0)), np.float32(np.nan)).astype(np.float32)
+
+
+def rmsnorm_int8(x: np.ndarray, w: np.ndarray, eps: float, delta: np.ndarray | None = None):
+    """(codes, scales, t): t = fp32(x + delta), the RMSNorm * (1 + w) of t in single fp32
+    roundings after a sum of squares in fp64, and its int8 rows. eps is taken as fp32."""
+    t = x.astype(np.float32) if delta is None else (x.astype(np.float32) + delta.astype(np.float32))
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        s = (t.astype(np.float64) ** 2).sum(axis=1) / t.shape[1] + np.float64(np.float32(eps))
+        r = (1.0 / np.sqrt(s)).astype(np.float32)
+        v = (t * r[:, None]) * (np.float32(1.0) + w.astype(np.float32))
+    q, scale = quantize_int8_rows(v)
+    return q, scale, t
+
+
+def int8_product(q: np.ndarray, scale: np.ndarray, w_codes: np.ndarray, w_scale: np.ndarray) -> np.ndarray:
+    """What the W8A8 linear computes, in float64 (integer sums up to 2^53 are exact there)."""
+    acc = q.astype(np.float64) @ w_codes.astype(np.float64).T
+    return acc * scale.astype(np.float64)[:, None] * w_scale.astype(np.float64)
+
+
 # ----------------------------------------------------------------------------- dispatch
 
-FORMATS = ("bf16", "int4", "nvfp4", "ternary")
+FORMATS = ("bf16", "int4", "nvfp4", "ternary", "int8")
 
 
 def dequantize(fmt: str, parts: dict) -> np.ndarray:
@@ -371,6 +414,8 @@ def dequantize(fmt: str, parts: dict) -> np.ndarray:
         return dequantize_nvfp4(parts["data"], parts["scales"], float(np.asarray(parts["global_scale"]).reshape(-1)[0]))
     if fmt == "ternary":
         return dequantize_ternary(parts["data"], parts["scales"])
+    if fmt == "int8":
+        return parts["data"].astype(np.float32) * parts["row_scale"][:, None]
     raise ValueError(fmt)
 
 
@@ -386,4 +431,7 @@ def quantize(fmt: str, w: np.ndarray) -> dict:
     if fmt == "ternary":
         d, s = quantize_ternary(w)
         return {"data": d, "scales": s}
+    if fmt == "int8":
+        d, s = quantize_int8_rows(w)
+        return {"data": d, "row_scale": s}
     raise ValueError(fmt)

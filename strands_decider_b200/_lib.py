@@ -20,9 +20,10 @@ LIB_PATH = _build.LIB
 B200_OK = 0
 STATUS = {1: "ARG", 2: "SHAPE", 3: "FORMAT", 4: "CUDA", 5: "WORKSPACE", 6: "TIMEOUT", 7: "UNSUPPORTED"}
 
-FMT = {"bf16": 0, "int4": 1, "nvfp4": 2, "ternary": 3}
+FMT = {"bf16": 0, "int4": 1, "nvfp4": 2, "ternary": 3, "int8": 4}
 EP_STORE, EP_RESID_ADD, EP_SWIGLU = 0, 1, 2
 LO_BF16, LO_E4M3 = 0, 1
+ACT_F32, ACT_BF16 = 0, 1
 LO8_X_SHIFT, LO8_W_SHIFT = 6, 6
 LO8_SHIFT = LO8_X_SHIFT + LO8_W_SHIFT
 LAYER_GDN, LAYER_ATTN = 0, 1
@@ -132,6 +133,9 @@ _SIGS = {
     "b200_quantize_act_nvfp4": ([_P, _I, _I, _I, _P, _P, _P], C.c_int),
     "b200_nvfp4_sf_atoms": ([_P, _I, _I, _P, _P], C.c_int),
     "b200_linear_nvfp4_native": ([_P, _P, _I, _I, C.POINTER(QWeight), _P, C.POINTER(LinearOut), _P], C.c_int),
+    "b200_quantize_act_int8": ([_P, _P, _I, _I, _I, _I, _P, _I, _P, _P], C.c_int),
+    "b200_rmsnorm_int8": ([_P, _I, _P, _I, _I, _P, _I, _I, _I, _P, C.c_float, _P, _I, _P, _P], C.c_int),
+    "b200_linear_int8": ([_P, _P, _I, _I, _I, C.POINTER(QWeight), C.POINTER(LinearOut), _P], C.c_int),
     "b200_decide_readout": ([_P, _I, _P, C.c_float, C.POINTER(Readout), C.POINTER(DecideArgs), _I, _P], C.c_int),
     "b200_model_create": ([C.POINTER(ModelConfig), C.POINTER(C.c_void_p)], C.c_int),
     "b200_model_destroy": ([_P], C.c_int),

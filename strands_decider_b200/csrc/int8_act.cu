@@ -1,0 +1,325 @@
+// Int8 codes with one fp32 scale per row: of an activation or a weight (b200_quantize_act_int8,
+// b200_quantize), and of a residual stream's RMSNorm (b200_rmsnorm_int8).
+//
+// Codes of a row v: a = max |v|, scale = a / 127, q = rint(v * (127 / a)), each operation one
+// fp32 rounding, so the codes are the same for every split of a row over threads; the norm's sum
+// of squares is taken in fp64, where the order of its additions does not show after the one
+// rounding of (S / hidden + eps)^-1/2 to fp32 (and no finite input overflows it). The maximum is
+// taken over the bit patterns of |v| as integers: a NaN or infinity then is the largest, and the
+// row gets scale NaN.
+//
+// Every row is read once: its elements stay in the registers of the threads that share it while
+// the sum, the maximum and the codes follow one another.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace sdb {
+
+constexpr int I8_K_MAX = 65536;  // also keeps b200_linear_int8's sums below 2^31
+
+// The reductions of one row over its TPR threads: a warp, or a whole block.
+template <int TPR>
+__device__ __forceinline__ double row_sum(double v, double* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0;
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) v += part[i];
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0u;
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) v = max(v, part[i]);
+  }
+  return v;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// A row's scale from the bits of its largest |v|, and the factor of its codes (0: all codes 0; a
+// NaN product converts to 0 too).
+__device__ __forceinline__ void row_scale(uint32_t amax_bits, float& scale, float& inv) {
+  scale = inv = 0.0f;
+  if (amax_bits >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fc00000u);
+    return;
+  }
+  const float a = __uint_as_float(amax_bits), s = __fdiv_rn(a, 127.0f);
+  if (s < 1.1754943508222875e-38f) return;  // 2^-126
+  scale = s;
+  inv = __fdiv_rn(127.0f, a);
+}
+
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+  const uint32_t q0 = uint32_t(__float2int_rn(__fmul_rn(a, inv))), q1 = uint32_t(__float2int_rn(__fmul_rn(b, inv)));
+  const uint32_t q2 = uint32_t(__float2int_rn(__fmul_rn(c, inv))), q3 = uint32_t(__float2int_rn(__fmul_rn(d, inv)));
+  return __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+}
+
+constexpr int ACT_NONE = -1, ACT_PLANES = 2;  // beside B200_ACT_F32 and B200_ACT_BF16
+
+struct RowArgs {
+  const void* x;        // quantise: fp32 or bf16; norm: fp32
+  const uint16_t* lo;   // quantise: the low plane
+  const void* delta;    // norm
+  float* sum;           // norm
+  const float* w;       // norm
+  int8_t* q;
+  float* scale;
+  int ldx, ldd, lds, ldq;
+  int rows, k;
+  float eps;
+};
+
+template <int TPR>
+__device__ __forceinline__ int row_of() {
+  return TPR == 32 ? int(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : int(blockIdx.x);
+}
+
+// TPR threads per row, NV float4 per thread (k <= 4 TPR NV).
+template <int TPR, int NV, int DELTA>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_int8_kernel(const RowArgs a) {
+  __shared__ double psum[TPR / 32];
+  __shared__ uint32_t pmax[TPR / 32];
+  pdl_wait();
+  pdl_trigger();
+  const int row = row_of<TPR>(), t = threadIdx.x % TPR;
+  if (row >= a.rows) return;
+  const int n4 = a.k / 4;
+  const float4* xr = reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + size_t(row) * a.ldx);
+  float4 v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = t + TPR * i;
+    v[i] = j < n4 ? xr[j] : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  if constexpr (DELTA != ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = t + TPR * i;
+      if (j < n4) {
+        float4 d;
+        if constexpr (DELTA == B200_ACT_F32) {
+          d = reinterpret_cast<const float4*>(static_cast<const float*>(a.delta) + size_t(row) * a.ldd)[j];
+        } else {
+          const uint2 b = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.delta) + size_t(row) * a.ldd)[j];
+          d = make_float4(bf16x2_lo(b.x), bf16x2_hi(b.x), bf16x2_lo(b.y), bf16x2_hi(b.y));
+        }
+        v[i] = make_float4(v[i].x + d.x, v[i].y + d.y, v[i].z + d.z, v[i].w + d.w);
+        if (a.sum) reinterpret_cast<float4*>(a.sum + size_t(row) * a.lds)[j] = v[i];
+      }
+    }
+  }
+  double ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    ss += double(v[i].x) * double(v[i].x);
+    ss += double(v[i].y) * double(v[i].y);
+    ss += double(v[i].z) * double(v[i].z);
+    ss += double(v[i].w) * double(v[i].w);
+  }
+  ss = row_sum<TPR>(ss, psum);
+  const float r = float(rsqrt(ss / double(a.k) + double(a.eps)));
+  uint32_t mx = 0u;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = t + TPR * i;
+    if (j < n4) {
+      const float4 w = __ldg(reinterpret_cast<const float4*>(a.w) + j);
+      v[i].x = __fmul_rn(__fmul_rn(v[i].x, r), 1.0f + w.x);
+      v[i].y = __fmul_rn(__fmul_rn(v[i].y, r), 1.0f + w.y);
+      v[i].z = __fmul_rn(__fmul_rn(v[i].z, r), 1.0f + w.z);
+      v[i].w = __fmul_rn(__fmul_rn(v[i].w, r), 1.0f + w.w);
+      mx = max(max(max(mx, abs_bits(v[i].x)), abs_bits(v[i].y)), max(abs_bits(v[i].z), abs_bits(v[i].w)));
+    }
+  }
+  mx = row_max<TPR>(mx, pmax);
+  float scale, inv;
+  row_scale(mx, scale, inv);
+  if (t == 0) a.scale[row] = scale;
+  uint32_t* qr = reinterpret_cast<uint32_t*>(a.q + size_t(row) * a.ldq);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = t + TPR * i;
+    if (j < n4) qr[j] = codes4(v[i].x, v[i].y, v[i].z, v[i].w, inv);
+  }
+}
+
+// TPR threads per row, NV groups of 4 (fp32) or 8 (bf16) elements per thread.
+template <int TPR, int NV, int TYPE>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_int8_kernel(const RowArgs a) {
+  constexpr int E = TYPE == B200_ACT_F32 ? 4 : 8;
+  __shared__ uint32_t pmax[TPR / 32];
+  pdl_wait();
+  pdl_trigger();
+  const int row = row_of<TPR>(), t = threadIdx.x % TPR;
+  if (row >= a.rows) return;
+  const int ng = a.k / E;
+  float v[NV][E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = t + TPR * i;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[i][e] = 0.0f;
+    if (j < ng) {
+      if constexpr (TYPE == B200_ACT_F32) {
+        const float4 f = reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + size_t(row) * a.ldx)[j];
+        v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
+      } else {
+        const uint4 h = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + size_t(row) * a.ldx)[j];
+        const uint32_t hw[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[i][2 * e] = bf16x2_lo(hw[e]);
+          v[i][2 * e + 1] = bf16x2_hi(hw[e]);
+        }
+        if constexpr (TYPE == ACT_PLANES) {
+          const uint4 l = reinterpret_cast<const uint4*>(a.lo + size_t(row) * a.ldx)[j];
+          const uint32_t lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[i][2 * e] += bf16x2_lo(lw[e]);
+            v[i][2 * e + 1] += bf16x2_hi(lw[e]);
+          }
+        }
+      }
+    }
+  }
+  uint32_t mx = 0u;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) mx = max(mx, abs_bits(v[i][e]));
+  mx = row_max<TPR>(mx, pmax);
+  float scale, inv;
+  row_scale(mx, scale, inv);
+  if (t == 0) a.scale[row] = scale;
+  int8_t* qr = a.q + size_t(row) * a.ldq;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = t + TPR * i;
+    if (j < ng) {
+      const uint32_t c = codes4(v[i][0], v[i][1], v[i][2], v[i][3], inv);
+      if constexpr (E == 4)
+        reinterpret_cast<uint32_t*>(qr)[j] = c;
+      else
+        reinterpret_cast<uint2*>(qr)[j] = make_uint2(c, codes4(v[i][4], v[i][5], v[i][6], v[i][7], inv));
+    }
+  }
+}
+
+// A block per row, of the fewest threads that hold it in 16 float4 each.
+template <int DELTA>
+static int launch_norm(const RowArgs& a, cudaStream_t st) {
+  const dim3 grid(a.rows);
+  if (a.k <= 4 * 128 * 16)
+    SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<128, 16, DELTA>, grid, dim3(128), 0, st, a));
+  else if (a.k <= 4 * 512 * 16)
+    SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<512, 16, DELTA>, grid, dim3(512), 0, st, a));
+  else
+    SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<1024, 16, DELTA>, grid, dim3(1024), 0, st, a));
+  return B200_OK;
+}
+
+template <int TYPE>
+static int launch_quant(const RowArgs& a, cudaStream_t st) {
+  constexpr int NV = TYPE == B200_ACT_F32 ? 16 : 8;
+  const dim3 grid(a.rows);
+  if (a.k <= 4 * 128 * 16)
+    SDB_CUDA(launch_pdl(quantize_int8_kernel<128, NV, TYPE>, grid, dim3(128), 0, st, a));
+  else if (a.k <= 4 * 512 * 16)
+    SDB_CUDA(launch_pdl(quantize_int8_kernel<512, NV, TYPE>, grid, dim3(512), 0, st, a));
+  else
+    SDB_CUDA(launch_pdl(quantize_int8_kernel<1024, NV, TYPE>, grid, dim3(1024), 0, st, a));
+  return B200_OK;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int sdb_quantize_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t rows, int32_t k, int32_t ldx,
+                      int8_t* q, int32_t ldq, float* scale, cudaStream_t st) {
+  if (!x || !q || !scale) return sdb_fail(B200_ERR_ARG, "b200_quantize_act_int8: null pointer");
+  if (type != B200_ACT_F32 && type != B200_ACT_BF16)
+    return sdb_fail(B200_ERR_ARG, "b200_quantize_act_int8: unknown activation type");
+  if (x_lo && type != B200_ACT_BF16)
+    return sdb_fail(B200_ERR_ARG, "b200_quantize_act_int8: a low plane belongs to bf16 activations");
+  if (rows <= 0 || k <= 0) return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: empty shape");
+  if (k % 16 != 0 || k > I8_K_MAX)
+    return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: k must be a multiple of 16, at most 65536");
+  if (ldx < k || ldx % (type == B200_ACT_F32 ? 4 : 8) != 0 || ldq < k || ldq % 16 != 0)
+    return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: row strides must hold k and be multiples of 16 bytes");
+  if (!aligned16(x) || !aligned16(x_lo) || !aligned16(q) || (reinterpret_cast<uintptr_t>(scale) & 3))
+    return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: x, x_lo and q must be 16-byte aligned");
+  RowArgs a{};
+  a.x = x;
+  a.lo = x_lo;
+  a.q = q;
+  a.scale = scale;
+  a.ldx = ldx;
+  a.ldq = ldq;
+  a.rows = rows;
+  a.k = k;
+  if (type == B200_ACT_F32) return launch_quant<B200_ACT_F32>(a, st);
+  return x_lo ? launch_quant<ACT_PLANES>(a, st) : launch_quant<B200_ACT_BF16>(a, st);
+}
+
+int sdb_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd, float* sum,
+                     int32_t lds, int32_t rows, int32_t hidden, const float* w, float eps, int8_t* q, int32_t ldq,
+                     float* scale, cudaStream_t st) {
+  if (!x || !w || !q || !scale) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: null pointer");
+  if (sum && !delta) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: sum needs a delta");
+  if (delta && delta_type != B200_ACT_F32 && delta_type != B200_ACT_BF16)
+    return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: unknown delta type");
+  if (!(eps >= 0.0f)) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: eps must not be negative");
+  if (rows <= 0 || hidden <= 0) return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: empty shape");
+  if (hidden % 16 != 0 || hidden > I8_K_MAX)
+    return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: hidden must be a multiple of 16, at most 65536");
+  if (ldx < hidden || ldx % 4 != 0 || ldq < hidden || ldq % 16 != 0 ||
+      (delta && (ldd < hidden || ldd % (delta_type == B200_ACT_F32 ? 4 : 8) != 0)) ||
+      (sum && (lds < hidden || lds % 4 != 0)))
+    return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: row strides must hold hidden and be multiples of 16 bytes");
+  if (!aligned16(x) || !aligned16(delta) || !aligned16(sum) || !aligned16(w) || !aligned16(q) ||
+      (reinterpret_cast<uintptr_t>(scale) & 3))
+    return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: x, delta, sum, w and q must be 16-byte aligned");
+  RowArgs a{};
+  a.x = x;
+  a.delta = delta;
+  a.sum = sum;
+  a.w = w;
+  a.q = q;
+  a.scale = scale;
+  a.ldx = ldx;
+  a.ldd = ldd;
+  a.lds = lds;
+  a.ldq = ldq;
+  a.rows = rows;
+  a.k = hidden;
+  a.eps = eps;
+  if (!delta) return launch_norm<ACT_NONE>(a, st);
+  return delta_type == B200_ACT_F32 ? launch_norm<B200_ACT_F32>(a, st) : launch_norm<B200_ACT_BF16>(a, st);
+}
+
+}  // namespace sdb
+
+extern "C" int b200_quantize_act_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t rows, int32_t k,
+                                      int32_t ldx, int8_t* q, int32_t ldq, float* scale, b200_stream stream) {
+  return sdb::sdb_quantize_int8(x, x_lo, type, rows, k, ldx, q, ldq, scale, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd,
+                                 float* sum, int32_t lds, int32_t rows, int32_t hidden, const float* w, float eps,
+                                 int8_t* q, int32_t ldq, float* scale, b200_stream stream) {
+  return sdb::sdb_rmsnorm_int8(x, ldx, delta, delta_type, ldd, sum, lds, rows, hidden, w, eps, q, ldq, scale,
+                               reinterpret_cast<cudaStream_t>(stream));
+}

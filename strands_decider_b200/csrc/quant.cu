@@ -179,6 +179,9 @@ __global__ void tile_kernel(b200_qweight w, uint8_t* __restrict__ tiles, uint8_t
   }
 }
 
+int sdb_quantize_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t rows, int32_t k, int32_t ldx,
+                      int8_t* q, int32_t ldq, float* scale, cudaStream_t st);
+
 }  // namespace sdb
 
 using namespace sdb;
@@ -200,6 +203,7 @@ extern "C" int b200_tile_weights(const b200_qweight* w, void* tiles, void* tile_
   if (!w || !w->data) return sdb_fail(B200_ERR_ARG, "b200_tile_weights: null pointer");
   if (w->n % 256 != 0 || w->k % 128 != 0) return sdb_fail(B200_ERR_SHAPE, "b200_tile_weights: bad shape");
   if (w->format == B200_W_BF16) return B200_OK;
+  if (w->format < 0 || w->format > 3) return sdb_fail(B200_ERR_FORMAT, "b200_tile_weights: format has no streaming copy");
   if (!tiles || (tile_scale_row_bytes(w->format) && !tile_scales))
     return sdb_fail(B200_ERR_ARG, "b200_tile_weights: null output");
   const long total = long(w->n) * (w->k / 64);
@@ -213,6 +217,12 @@ extern "C" int b200_quantize(int32_t format, const float* w, int32_t n, int32_t 
                              float* row_scale, b200_stream stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (!w || !data || n <= 0 || k <= 0) return sdb_fail(B200_ERR_ARG, "b200_quantize: null pointer or empty shape");
+  if (format == B200_W_INT8) {  // a weight row takes its codes as an activation row does
+    if (!row_scale) return sdb_fail(B200_ERR_ARG, "b200_quantize: int8 needs row_scale");
+    const int rc = sdb_quantize_int8(w, nullptr, B200_ACT_F32, n, k, k, static_cast<int8_t*>(data), k, row_scale, st);
+    if (rc != B200_OK) sdb_rename_error("b200_quantize_act_int8:", "b200_quantize:");
+    return rc;
+  }
   if (k % 128 != 0) return sdb_fail(B200_ERR_SHAPE, "b200_quantize: k must be a multiple of 128");
   switch (format) {
     case B200_W_INT4G128: {

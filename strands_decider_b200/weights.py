@@ -35,7 +35,7 @@ class PackedWeight:
 
     def ensure_tiles(self) -> None:
         """Build the per-(256-row tile, 64-column stage) streaming copy the GEMM reads."""
-        if self.fmt == "bf16" or self.tiles is not None or self.n % 256 != 0:
+        if self.fmt in ("bf16", "int8") or self.tiles is not None or self.n % 256 != 0:
             return
         tb, sb = C.c_size_t(), C.c_size_t()
         _lib.check(_lib.load().b200_tile_bytes(_lib.FMT[self.fmt], self.n, self.k, C.byref(tb), C.byref(sb)))
@@ -90,10 +90,14 @@ def quantize(fmt: str, w: torch.Tensor, stream: torch.cuda.Stream | None = None)
         data = torch.empty(n, k // 4, dtype=torch.uint8, device=dev)
         scales = torch.empty(n, dtype=torch.int16, device=dev)
         row_scale = None
+    elif fmt == "int8":
+        data = torch.empty(n, k, dtype=torch.int8, device=dev)
+        scales = None
+        row_scale = torch.empty(n, dtype=torch.float32, device=dev)
     else:
         raise ValueError(f"unknown weight format {fmt!r}")
     _lib.call("b200_quantize", _lib.FMT[fmt], _lib.ptr(w), n, k, _lib.ptr(data), _lib.ptr(scales),
-              _lib.ptr(row_scale) if row_scale is not None else None, _lib.stream_ptr(stream))
+              _lib.ptr(row_scale), _lib.stream_ptr(stream))
     return PackedWeight(fmt, n, k, data, scales, row_scale)
 
 
@@ -271,7 +275,9 @@ def packed_to_numpy(pw: PackedWeight) -> dict:
     if pw.scales is not None:
         s = pw.scales.cpu().numpy()
         out["scales"] = s.view(np.uint16) if s.dtype == np.int16 else s
-    if pw.row_scale is not None:
+    if pw.fmt == "int8":
+        out["row_scale"] = pw.row_scale.cpu().numpy()
+    elif pw.row_scale is not None:
         out["global_scale"] = pw.row_scale[:1].cpu().numpy()
     return out
 

@@ -1,0 +1,467 @@
+"""The int8 (W8A8) operators against plain implementations in 64 bits.
+
+* Codes and scales (b200_quantize_act_int8, b200_rmsnorm_int8, b200_quantize): equal to
+  oracle.quant's, every step of which is one fp32 rounding.
+* The product (b200_linear_int8): against the fp64 product of the codes. The int32 sum is exact,
+  so a stored output has three roundings (sum to fp32, two scales): |y - ref| <= 3 * 2^-24 |ref|
+  to first order, tested with 4 * 2^-24. A residual adds one rounding of the result.
+* The SwiGLU: g, u as above; silu by the fast exponential and division: relative error at most
+  (2 + 1.2 |g|) * 2^-23 (exponential), 2 * 2^-23 (division), 3 * 2^-24 |g| (g's own error through
+  the exponent), and the roundings of 1 + e and of the products, in all below 2^-17 for |g| <= 20;
+  then a plane's rounding: 2^-8 for the hi plane alone, 2^-16 for hi + bf16 lo, and for an e4m3 lo
+  plane 2^-4 of |h - hi| <= 2^-8 |h|, or half a step of its subnormals, 2^-10 / 2^6.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import quant as Q
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("the -m gpu tests need a CUDA device")
+    from strands_decider_b200 import _lib
+
+    _lib.load()
+    yield
+    torch.cuda.synchronize()
+    assert _lib.read_fault() == 0
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _same_codes(q, scale, want_q, want_s):
+    assert np.array_equal(scale.cpu().numpy(), want_s, equal_nan=True)
+    assert np.array_equal(q.cpu().numpy(), want_q)
+
+
+def _hard_rows(rows, k, seed):
+    """Rows of varied size, with the ones a quantiser can get wrong in front."""
+    x = torch.randn(rows, k, generator=_gen(seed)) * torch.exp(3 * torch.randn(rows, 1, generator=_gen(seed + 1)))
+    hard = [torch.zeros(k), torch.full((k,), 3.0), torch.full((k,), 1e-45), torch.full((k,), 1.4e-36),
+            torch.full((k,), 3e38), torch.arange(k).float() - k / 2]
+    spike = torch.full((k,), 1e-30)
+    spike[k - 1] = -1e30
+    ties = torch.zeros(k)            # half codes: 0.5, 1.5, 2.5, ... of a scale of exactly 1
+    ties[0] = 127.0
+    ties[1:8] = torch.tensor([0.5, 1.5, 2.5, -0.5, -1.5, 63.5, -126.5])
+    inf = torch.randn(k, generator=_gen(seed + 2))
+    inf[k // 2] = float("-inf")
+    nan = torch.randn(k, generator=_gen(seed + 3))
+    nan[0] = float("nan")
+    for i, h in enumerate(hard + [spike, ties, inf, nan]):
+        if rows > 2 * i:
+            x[2 * i] = h
+    return x
+
+
+ROW_SHAPES = [(1, 16), (1, 2048), (1, 6144), (3, 48), (5, 1040), (21, 2032), (33, 4096), (23, 8208), (4, 32784),
+              (2, 65536), (1500, 144), (4099, 1152)]
+
+
+@pytest.mark.parametrize("rows,k", ROW_SHAPES)
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "planes"])
+def test_quantize_act_is_exact(rows, k, kind):
+    from strands_decider_b200 import int8
+
+    x = _hard_rows(rows, k, rows + k)
+    lo = None
+    if kind == "fp32":
+        want = x
+    else:
+        hi = x.to(torch.bfloat16)
+        want = hi.float()
+        if kind == "planes":
+            lo = (x - want).to(torch.bfloat16)
+            want = want + lo.float()
+        x = hi
+    q, s = int8.quantize_act(x.cuda(), lo=lo.cuda() if lo is not None else None)
+    _same_codes(q, s, *Q.quantize_int8_rows(want.numpy()))
+
+
+@pytest.mark.parametrize("rows,k", ROW_SHAPES)
+@pytest.mark.parametrize("delta", [None, torch.float32, torch.bfloat16])
+def test_rmsnorm_is_exact(rows, k, delta):
+    from strands_decider_b200 import int8
+
+    x = _hard_rows(rows, k, rows + k + 1)
+    w = torch.randn(k, generator=_gen(k)) * 0.2
+    d = None if delta is None else torch.randn(rows, k, generator=_gen(7)).to(delta)
+    want_q, want_s, want_t = Q.rmsnorm_int8(x.numpy(), w.numpy(), 1e-6, None if d is None else d.float().numpy())
+    t = torch.empty(rows, k, device="cuda") if d is not None else None
+    q, s = int8.rmsnorm(x.cuda(), w.cuda(), 1e-6, delta=d.cuda() if d is not None else None, resid_out=t)
+    _same_codes(q, s, want_q, want_s)
+    if t is not None:
+        assert np.array_equal(t.cpu().numpy(), want_t, equal_nan=True)
+
+
+def test_rmsnorm_in_place_and_without_a_sum():
+    """The sum may land in x or in an fp32 delta, or nowhere; the codes are the same."""
+    from strands_decider_b200 import int8
+
+    x, d = torch.randn(37, 528).cuda(), torch.randn(37, 528).cuda()
+    w = torch.randn(528).cuda()
+    q0, s0 = int8.rmsnorm(x, w, 1e-5, delta=d)
+    t = x + d
+    x1, d1 = x.clone(), d.clone()
+    q1, s1 = int8.rmsnorm(x1, w, 1e-5, delta=d, resid_out=x1)
+    q2, s2 = int8.rmsnorm(x, w, 1e-5, delta=d1, resid_out=d1)
+    for q, s in ((q1, s1), (q2, s2)):
+        assert torch.equal(q, q0) and torch.equal(s, s0)
+    assert torch.equal(x1, t) and torch.equal(d1, t)
+
+
+def test_row_strides_and_what_lies_between_rows():
+    """Views with a row stride read and write their own columns only."""
+    from strands_decider_b200 import int8
+
+    rows, k = 19, 272
+    x = torch.full((rows, 400), float("nan")).cuda()
+    x[:, 64:64 + k] = torch.randn(rows, k).cuda()
+    q = torch.full((rows, 512), 99, dtype=torch.int8).cuda()
+    s = torch.full((rows + 2,), -7.0).cuda()
+    int8.quantize_act(x[:, 64:64 + k], out=q[:, 128:128 + k], scale=s[1:-1])
+    _same_codes(q[:, 128:128 + k], s[1:-1], *Q.quantize_int8_rows(x[:, 64:64 + k].cpu().numpy()))
+    assert (q[:, :128] == 99).all() and (q[:, 128 + k:] == 99).all() and s[0] == -7 and s[-1] == -7
+    t = torch.full((rows, 300), 5.0).cuda()
+    d = torch.randn(rows, 320).to(torch.bfloat16).cuda()
+    w = torch.randn(k).cuda()
+    int8.rmsnorm(x[:, 64:64 + k], w, 1e-6, delta=d[:, 16:16 + k], resid_out=t[:, 12:12 + k], out=q[:, 16:16 + k],
+                 scale=s[:rows])
+    wq, ws, wt = Q.rmsnorm_int8(x[:, 64:64 + k].cpu().numpy(), w.cpu().numpy(), 1e-6,
+                                d[:, 16:16 + k].float().cpu().numpy())
+    _same_codes(q[:, 16:16 + k], s[:rows], wq, ws)
+    assert np.array_equal(t[:, 12:12 + k].cpu().numpy(), wt)
+    assert (t[:, :12] == 5).all() and (t[:, 12 + k:] == 5).all()
+
+
+@pytest.mark.parametrize("n,k", [(1, 16), (300, 2048), (129, 4112)])
+def test_weight_quantiser_is_exact(n, k):
+    from strands_decider_b200 import weights as W
+
+    w = _hard_rows(n, k, 3) if n > 30 else torch.randn(n, k)
+    pw = W.quantize("int8", w.cuda())
+    parts = W.packed_to_numpy(pw)
+    want = Q.quantize("int8", w.numpy())
+    assert np.array_equal(parts["data"], want["data"])
+    assert np.array_equal(parts["row_scale"], want["row_scale"], equal_nan=True)
+
+
+# ----------------------------------------------------------------------------- the product
+
+
+def _operands(m, n, k, seed):
+    g = _gen(seed)
+    q = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+    wq = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8)
+    s = torch.exp(torch.randn(m, generator=g)) / 1024
+    ws = torch.exp(torch.randn(n, generator=g)) / 1024
+    return q, s, wq, ws
+
+
+def _weight(wq, ws):
+    from strands_decider_b200.weights import PackedWeight
+
+    return PackedWeight("int8", wq.shape[0], wq.shape[1], wq.cuda(), row_scale=ws.cuda())
+
+
+def _ref(q, s, wq, ws):
+    """fp64 on the GPU (exact sums of whole numbers below 2^53)."""
+    return ((q.cuda().double() @ wq.cuda().double().T) * s.cuda().double()[:, None]) * ws.cuda().double()
+
+
+# one row to several tiles; outputs that are no multiple of anything; depths that end inside a tile
+SHAPES = [(1, 1, 16), (1, 130, 64), (2, 2048, 2048), (7, 1000, 144), (8, 96, 8208), (9, 257, 1040), (16, 2304, 512),
+          (17, 640, 2048), (31, 33, 48), (33, 129, 6144), (64, 1153, 528), (65, 256, 4112), (96, 8224, 256),
+          (127, 384, 1024), (129, 127, 272), (200, 2048, 2032), (255, 600, 2064), (257, 520, 128), (511, 1025, 400),
+          (1021, 2048, 2048), (2050, 4200, 336), (4099, 2600, 1040)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear_store_and_residual(m, n, k):
+    from strands_decider_b200 import int8
+
+    q, s, wq, ws = _operands(m, n, k, m + n + k)
+    w = _weight(wq, ws)
+    ref = _ref(q, s, wq, ws)
+    out = torch.full((m, n), 7.0, device="cuda")
+    int8.linear(q.cuda(), s.cuda(), w, out)
+    assert ((out.double() - ref).abs() <= 4 * U * ref.abs()).all()
+    out = torch.randn(m, n, device="cuda") * ref.abs().mean().float()
+    want = out.double() + ref
+    int8.linear(q.cuda(), s.cuda(), w, out, epilogue="residual")
+    assert ((out.double() - want).abs() <= 4 * U * ref.abs() + 1.01 * U * want.abs()).all()
+
+
+SWIGLU_SHAPES = [(1, 128, 16), (1, 12288, 256), (5, 256, 144), (13, 1152, 2048), (16, 128, 1040), (24, 640, 528),
+                 (96, 1024, 2048), (130, 384, 400), (300, 2432, 1024), (1030, 1280, 272), (2050, 4224, 160)]
+
+
+@pytest.mark.parametrize("m,n,k", SWIGLU_SHAPES)
+@pytest.mark.parametrize("lo", [None, "bf16", "e4m3"])
+def test_linear_swiglu(m, n, k, lo):
+    from strands_decider_b200 import int8
+
+    q, s, wq, ws = _operands(m, n, k, m + n)
+    # |g|, |u| up to about 20: the codes' products have a standard deviation of 74^2 sqrt(k)
+    s = torch.full((m,), 4.0 / (74.0 ** 2 * k ** 0.5))
+    ws = torch.exp(0.2 * torch.randn(n, generator=_gen(n)))
+    y = _ref(q, s, wq, ws).reshape(m, -1, 2, 64)
+    g, u = y[:, :, 0], y[:, :, 1]
+    ref = (g * torch.sigmoid(g) * u).reshape(m, n // 2)
+    out = torch.zeros(m, n // 2, dtype=torch.bfloat16, device="cuda")
+    lo_t = None
+    if lo is not None:
+        lo_t = torch.zeros(m, n // 2, dtype=torch.bfloat16 if lo == "bf16" else torch.float8_e4m3fn, device="cuda")
+    int8.linear(q.cuda(), s.cuda(), _weight(wq, ws), out, epilogue="swiglu", lo=lo_t)
+    got = out.double()
+    assert g.abs().max() < 32
+    fast = 2.0 ** -17 + g.abs().max().item() * 2.0 ** -22
+    tol = (2.0 ** -8 + fast) * ref.abs()
+    assert ((got - ref).abs() <= tol).all()
+    if lo == "bf16":
+        got = got + lo_t.double()
+        tol = (2.0 ** -16 + 2 * fast) * ref.abs()
+    elif lo == "e4m3":
+        got = got + lo_t.double() / 64
+        tol = (2.0 ** -12 + 2 * fast) * ref.abs() + 2.0 ** -16
+    assert ((got - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m", [1, 12, 40, 300])
+def test_linear_extreme_codes_at_the_greatest_depth(m):
+    """-128 x -128 over k = 65536 is 2^30; signs and single codes come through exactly."""
+    from strands_decider_b200 import int8
+
+    k, n = 65536, 130
+    q = torch.full((m, k), -128, dtype=torch.int8)
+    wq = torch.full((n, k), -128, dtype=torch.int8)
+    wq[1::3] = 127
+    wq[2::3] = 0
+    wq[2::3, 5] = 1
+    q[m // 2] = 127
+    out = torch.empty(m, n, device="cuda")
+    int8.linear(q.cuda(), torch.ones(m, device="cuda"), _weight(wq, torch.ones(n)), out)
+    assert torch.equal(out.double(), _ref(q, torch.ones(m), wq, torch.ones(n)).float().double())
+
+
+@pytest.mark.parametrize("m,k", [(3, 256), (30, 2048), (140, 272), (700, 128)])
+def test_linear_strides_partial_outputs_and_neighbours(m, k):
+    """A strided q, fewer outputs than weight rows, a wider out: nothing else is touched."""
+    from strands_decider_b200 import int8
+
+    n, nv = 700, 443
+    q, s, wq, ws = _operands(m, n, k, 5)
+    big = torch.full((m, k + 48), 77, dtype=torch.int8).cuda()
+    big[:, 16:16 + k] = q.cuda()
+    out = torch.full((m + 2, 500), 3.0).cuda()
+    int8.linear(big[:, 16:16 + k], s.cuda(), _weight(wq, ws), out[1:-1, 5:5 + nv], n_valid=nv)
+    ref = _ref(q, s, wq, ws)[:, :nv]
+    assert ((out[1:-1, 5:5 + nv].double() - ref).abs() <= 4 * U * ref.abs()).all()
+    assert (out[0] == 3).all() and (out[-1] == 3).all() and (out[:, :5] == 3).all() and (out[:, 5 + nv:] == 3).all()
+    h = torch.full((m + 2, 400), 2.0, dtype=torch.bfloat16).cuda()
+    s8 = torch.full((m,), 4.0 / (74.0 ** 2 * k ** 0.5)).cuda()
+    int8.linear(big[:, 16:16 + k], s8, _weight(wq, torch.ones(n)), h[1:-1, 3:3 + 192], epilogue="swiglu", n_valid=384)
+    y = _ref(q, s8, wq, torch.ones(n))[:, :384].reshape(m, 3, 2, 64)
+    ref = (torch.nn.functional.silu(y[:, :, 0]) * y[:, :, 1]).reshape(m, 192)
+    assert ((h[1:-1, 3:195].double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -16) * ref.abs()).all()
+    assert (h[0] == 2).all() and (h[-1] == 2).all() and (h[:, :3] == 2).all() and (h[:, 195:] == 2).all()
+
+
+@pytest.mark.parametrize("ep", ["store", "swiglu"])
+def test_a_row_does_not_depend_on_its_batch(ep):
+    """Bit for bit the same row alone, in small, middle and large batches, and run to run."""
+    from strands_decider_b200 import int8
+
+    m, n, k = 1200, 768, 1040
+    q, s, wq, ws = _operands(m, n, k, 11)
+    s = s * 0.01
+    w = _weight(wq, ws)
+    q, s = q.cuda(), s.cuda()
+
+    def run(a, b):
+        out = torch.empty(b - a, n if ep == "store" else n // 2, device="cuda",
+                          dtype=torch.float32 if ep == "store" else torch.bfloat16)
+        return int8.linear(q[a:b], s[a:b], w, out, epilogue=ep)
+
+    whole = run(0, m)
+    assert torch.equal(whole, run(0, m))
+    for a, b in ((0, 1), (5, 12), (3, 19), (100, 133), (0, 64), (200, 300), (0, 129), (400, 700)):
+        assert torch.equal(run(a, b), whole[a:b]), (a, b)
+
+
+def test_a_row_that_is_not_finite_stays_alone():
+    from strands_decider_b200 import int8
+
+    for m in (5, 50, 500):
+        x = torch.randn(m, 256)
+        x[3, 7] = float("inf")
+        q, s = int8.quantize_act(x.cuda())
+        _, _, wq, ws = _operands(1, 320, 256, 2)
+        out = torch.empty(m, 320, device="cuda")
+        int8.linear(q, s, _weight(wq, ws), out)
+        bad = torch.isnan(out)
+        assert bad[3].all() and not bad[:3].any() and not bad[4:].any()
+        resid = torch.zeros(m, 320, device="cuda")
+        int8.linear(q, s, _weight(wq, ws), resid, epilogue="residual")
+        assert torch.isnan(resid[3]).all() and not torch.isnan(resid[4:]).any()
+
+
+def test_output_offsets_past_32_bits():
+    """An out whose last row starts past 2^31 elements."""
+    from strands_decider_b200 import int8
+
+    for m in (4, 40, 300):
+        ld = (1 << 31) // (m - 1) + 64
+        out = torch.empty((m - 1) * ld + 256, device="cuda")
+        view = out.as_strided((m, 256), (ld, 1))
+        q, s, wq, ws = _operands(m, 256, 64, m)
+        int8.linear(q.cuda(), s.cuda(), _weight(wq, ws), view)
+        ref = _ref(q, s, wq, ws)
+        assert ((view.double() - ref).abs() <= 4 * U * ref.abs()).all()
+        del out, view
+
+
+# ----------------------------------------------------------------------------- together, as they are used
+
+
+def _mlp(x, delta, p, bufs):
+    """The MLP half of a layer: x += delta, norm, gate / up, SwiGLU, down, back into x."""
+    from strands_decider_b200 import int8
+
+    q, s = int8.rmsnorm(x, p["norm"], 1e-6, delta=delta, resid_out=x, out=bufs["q"], scale=bufs["s"])
+    int8.linear(q, s, p["gate_up"], bufs["h"], epilogue="swiglu")
+    hq, hs = int8.quantize_act(bufs["h"], out=bufs["hq"], scale=bufs["hs"])
+    return int8.linear(hq, hs, p["down"], x, epilogue="residual")
+
+
+def _mlp_setup(m, hidden=512, inter=1088):
+    from strands_decider_b200 import weights as W
+
+    g = torch.Generator(device="cuda").manual_seed(m)
+
+    def randn(*shape):
+        return torch.randn(*shape, device="cuda", generator=g)
+
+    gate, up, down = randn(inter, hidden) * 0.05, randn(inter, hidden) * 0.05, randn(hidden, inter) * 0.05
+    p = {"norm": randn(hidden) * 0.1, "w": (gate, up, down),
+         "gate_up": W.interleave_gate_up(W.quantize("int8", gate), W.quantize("int8", up)),
+         "down": W.concat_rows([W.quantize("int8", down)])}
+    n = 2 * inter
+    bufs = {"q": torch.empty(m, hidden, dtype=torch.int8, device="cuda"), "s": torch.empty(m, device="cuda"),
+            "h": torch.empty(m, inter, dtype=torch.bfloat16, device="cuda"),
+            "hq": torch.empty(m, inter, dtype=torch.int8, device="cuda"), "hs": torch.empty(m, device="cuda")}
+    assert p["gate_up"].n >= n
+    p["gate_up"] = W.PackedWeight("int8", n, hidden, p["gate_up"].data[:n].contiguous(),
+                                  row_scale=p["gate_up"].row_scale[:n].contiguous())
+    return p, bufs, randn(m, hidden), randn(m, hidden)
+
+
+@pytest.mark.parametrize("m", [1, 16, 77, 1000])
+def test_mlp_of_the_operators(m):
+    """Against the same chain in 64 bits on the device's own codes, step by step exact; and near
+    the unquantised MLP: rounding to codes is off by amax / 127 / sqrt(12) in the mean square, and
+    a row's amax is at most about 10 of its standard deviations (4 for a Gaussian row, more for
+    the SwiGLU's products)."""
+    from strands_decider_b200 import weights as W
+
+    p, bufs, x, delta = _mlp_setup(m)
+    t = x + delta
+    got = _mlp(x.clone(), delta, p, bufs)
+    q, s, _ = Q.rmsnorm_int8(x.cpu().numpy(), p["norm"].cpu().numpy(), 1e-6, delta.cpu().numpy())
+    _same_codes(bufs["q"], bufs["s"], q, s)
+    parts = W.packed_to_numpy(p["gate_up"])
+    y = torch.from_numpy(Q.int8_product(q, s, parts["data"], parts["row_scale"])).reshape(m, -1, 2, 64)
+    h = (torch.nn.functional.silu(y[:, :, 0]) * y[:, :, 1]).reshape(m, -1)
+    assert ((bufs["h"].double().cpu() - h).abs() <= (2.0 ** -8 + 2.0 ** -16) * h.abs()).all()
+    hq, hs = Q.quantize_int8_rows(bufs["h"].float().cpu().numpy())
+    _same_codes(bufs["hq"], bufs["hs"], hq, hs)
+    parts = W.packed_to_numpy(p["down"])
+    ref = torch.from_numpy(Q.int8_product(hq, hs, parts["data"], parts["row_scale"]))
+    want = t.double().cpu() + ref
+    assert ((got.double().cpu() - want).abs() <= 4 * U * ref.abs() + 1.01 * U * want.abs()).all()
+    gate, up, down = (w.double() for w in p["w"])
+    v = t.double() * torch.rsqrt(t.double().square().mean(-1, keepdim=True) + 1e-6) * (1 + p["norm"].double())
+    full = (torch.nn.functional.silu(v @ gate.T) * (v @ up.T)) @ down.T
+    off = (got.double() - t.double() - full).norm() / full.norm()
+    # six quantised operands, independent; the SiLU's slope is at most 1.1
+    assert off < 6 ** 0.5 * 1.1 * 10 / 127 / 12 ** 0.5
+
+
+def test_mlp_captured_replayed_and_on_two_streams():
+    """A captured chain replays on new inputs; two chains on two streams do not meet."""
+    sets = [_mlp_setup(m) for m in (9, 150)]
+    want = [_mlp(x.clone(), d, p, b).clone() for p, b, x, d in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    xs = [x.clone() for _, _, x, _ in sets]
+    for _ in range(5):
+        for i, (p, b, x, d) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                xs[i].copy_(x)
+                _mlp(xs[i], d, p, b)
+    torch.cuda.synchronize()
+    assert torch.equal(xs[0], want[0]) and torch.equal(xs[1], want[1])
+    for i, (p, b, x, d) in enumerate(sets):
+        buf, dd = x.clone(), d.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            _mlp(buf, dd, p, b)
+        torch.cuda.synchronize()
+        assert torch.equal(buf, x)       # capturing runs nothing
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(buf, want[i])
+        x2, d2 = torch.randn_like(x), torch.randn_like(d)
+        buf.copy_(x2)
+        dd.copy_(d2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(buf, _mlp(x2.clone(), d2, p, b))
+
+
+def test_python_operators_refuse_before_launching():
+    from strands_decider_b200 import _lib, int8
+    from strands_decider_b200 import weights as W
+
+    x = torch.zeros(4, 64, device="cuda")
+    w = W.quantize("int8", torch.randn(128, 64, device="cuda"))
+    q, s = int8.quantize_act(x)
+    out = torch.zeros(4, 128, device="cuda")
+    for bad in (lambda: int8.quantize_act(x.half()), lambda: int8.quantize_act(x[0]),
+                lambda: int8.quantize_act(x, lo=x), lambda: int8.quantize_act(x.t()),
+                lambda: int8.quantize_act(x, out=torch.empty(4, 64, device="cuda")),
+                lambda: int8.quantize_act(x, scale=torch.empty(5, device="cuda")),
+                lambda: int8.quantize_act(x, scale=torch.empty(4)),
+                lambda: int8.rmsnorm(x, torch.zeros(32, device="cuda"), 1e-6),
+                lambda: int8.rmsnorm(x, torch.zeros(64, device="cuda"), 1e-6, resid_out=x),
+                lambda: int8.rmsnorm(x, torch.zeros(64, device="cuda"), 1e-6, delta=x.double()),
+                lambda: int8.linear(q, s, W.quantize("int4", torch.zeros(256, 128, device="cuda")), out),
+                lambda: int8.linear(q, s, w, out, epilogue="gelu"),
+                lambda: int8.linear(q, s, w, out, lo=out),
+                lambda: int8.linear(q, s, w, out.to(torch.bfloat16)),
+                lambda: int8.linear(q, s, w, out[:, :100]),
+                lambda: int8.linear(q, s[:3], w, out),
+                lambda: int8.linear(x, s, w, out),
+                lambda: int8.linear(q, s, w, out, epilogue="swiglu")):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: int8.quantize_act(x[:, :40]), lambda: int8.quantize_act(x[:0]),
+                lambda: int8.rmsnorm(x, torch.zeros(64, device="cuda"), -1.0),
+                lambda: int8.linear(q[:, :48], s, w, out)):
+        with pytest.raises(_lib.B200Error):
+            bad()
+    assert (out == 0).all()
