@@ -1,5 +1,18 @@
 // W8A8 linears: y[t, n] = (sum_k q[t, k] w[n, k]) * scale[t] * row_scale[n], int32 sums.
+//
+// Every kernel here takes the weight rows as the tensor core's M operand and the tokens as its N
+// operand, so an accumulator's lane is an output feature: 32 lanes write 32 neighbouring outputs of
+// one token, whatever the row stride and however many outputs there are, and the channel scale is
+// one register per lane. The int32 sum does not depend on the order of its terms and the two
+// scales are applied in one order (i8_value), so a row's result is the same bits in every kernel,
+// batch and split.
+//
+//   gemm_i8_pair_kernel   CTA pairs, 256 features x 256 tokens, persistent (large products)
+//   gemm_i8_split_kernel  one CTA per 128 features x up to 128 tokens and K range; the K ranges of
+//                         a tile are a cluster that adds its sums through distributed shared memory
+//   gemm_i8_reg_kernel    at most 16 tokens: weights through registers into mma.sync
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -12,15 +25,22 @@ struct I8Args {
   const float* ws;      // [n]
   b200_linear_out o;
   int m, n, k, ldx;
+  int ngroup;           // pair kernel: feature tiles per group
+  int bt, stages, split;  // split kernel: tokens per tile, ring depth, CTAs per tile
 };
 
-// The SwiGLU's output at token t, feature f: silu(g) * u as the bf16 hi plane and, if asked, the
-// low plane.
-__device__ __forceinline__ void store_swiglu(const b200_linear_out& o, int t, int f, float g, float u) {
-  const float h = silu_approx(g) * u;
+constexpr int I8_BK = 128;  // bytes (= codes) of K per stage: one 128-byte swizzled row
+
+__device__ __forceinline__ float i8_value(int acc, float xs, float ws) {
+  return __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws);
+}
+
+// The SwiGLU's output at element idx of the planes: silu(g) * u as the bf16 hi plane and, if
+// asked, the low plane.
+__device__ __forceinline__ void store_swiglu(const b200_linear_out& o, size_t idx, float g, float u) {
+  const float h = __fmul_rn(silu_approx(g), u);
   const uint16_t hb = f32_to_bf16_rn(h);
   uint16_t* dst = static_cast<uint16_t*>(o.out);
-  const size_t idx = size_t(t) * o.ldo + f;
   dst[idx] = hb;
   if (!o.lo_offset) return;
   if (o.lo_format == B200_LO_E4M3)
@@ -29,46 +49,647 @@ __device__ __forceinline__ void store_swiglu(const b200_linear_out& o, int t, in
     dst[o.lo_offset + idx] = f32_to_bf16_rn(h - bf16_to_f32(hb));
 }
 
-// One thread per output: 4 products per dp4a, straight from global memory.
-__device__ __forceinline__ float dot_int8(const I8Args& a, int t, int n) {
-  const int4* x = reinterpret_cast<const int4*>(a.q + size_t(t) * a.ldx);
-  const int4* w = reinterpret_cast<const int4*>(a.w + size_t(n) * a.k);
-  int acc = 0;
-  for (int i = 0; i < a.k / 16; ++i) {
-    const int4 p = x[i], r = __ldg(w + i);
-    acc = __dp4a(p.x, r.x, acc);
-    acc = __dp4a(p.y, r.y, acc);
-    acc = __dp4a(p.z, r.z, acc);
-    acc = __dp4a(p.w, r.w, acc);
+// Instruction descriptor, kind::i8: D s32, A and B signed bytes, both K-major, M x N.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
+// ----------------------------------------------------------------------------- CTA pairs
+// Tile: 256 features (128 per CTA) x 256 tokens, K in stages of 128 codes (four MMAs of K = 32).
+// Each CTA loads its 128 weight rows and its half of the tokens; the pair's MMA reads both halves.
+//   warp 0      TMA ring (both CTAs; bytes signalled on the leader's full barrier)
+//   warp 1      the leader's lane 0 issues the MMAs into one of two 256-column accumulators
+//   warps 2..9  epilogue: TMEM lane quarter warp % 4, token half (warp - 2) / 4
+constexpr int I8P_THREADS = 320;
+constexpr int I8P_EPI_WARPS = 8;
+
+template <int EP>
+struct I8PairSmem {
+  static constexpr int OP = 128 * I8_BK;                    // one operand of a stage
+  static constexpr int STAGE = 2 * OP;
+  // the SwiGLU gives one stage for the exchange of gate and up sums between lane halves
+  static constexpr int STAGES = EP == B200_EP_SWIGLU ? 5 : 6;
+  static constexpr int XCH = EP == B200_EP_SWIGLU ? 4 * 2 * 32 * 32 * 4 : 0;
+  static constexpr int XS = I8P_EPI_WARPS * 64 * 4;         // each epilogue warp's token scales
+  static constexpr int BARS = 2 * STAGES + 4;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE + XCH + XS + BARS * 8 + 16;
+  static_assert(TOTAL <= 227 * 1024, "shared memory");
+};
+
+template <int EP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
+    gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                        const I8Args a) {
+  using SM = I8PairSmem<EP>;
+  extern __shared__ uint8_t i8_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sX = sW + SM::STAGES * SM::OP;
+  float* xch = reinterpret_cast<float*>(sX + SM::STAGES * SM::OP);
+  float* sxs = xch + SM::XCH / 4;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sxs + SM::XS / 4);
+  uint64_t* full = bars;                            // the leader's are used
+  uint64_t* empty = bars + SM::STAGES;              // both CTAs'
+  uint64_t* acc_full = bars + 2 * SM::STAGES;       // [2], both CTAs'
+  uint64_t* acc_empty = bars + 2 * SM::STAGES + 2;  // [2], the leader's are used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SM::BARS);
+
+  const uint32_t rank = cluster_ctarank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nk = (a.k + I8_BK - 1) / I8_BK;
+  const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + 255) / 256;
+  const int n_units = n_tiles * m_tiles;
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  // groups of ngroup feature tiles; token tiles within a group, so that the weights a group
+  // re-reads stay in L2 while the activations stream past
+  const int G = a.ngroup;
+  auto tile_of = [&](int u, int& mt, int& nt) {
+    const int g = u / (G * m_tiles), r = u - g * G * m_tiles;
+    const int gs = min(G, n_tiles - g * G);
+    mt = r / gs;
+    nt = g * G + r % gs;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SM::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * I8P_EPI_WARPS);
+    }
+    mbar_fence_init();
   }
-  return float(acc) * a.xs[t] * a.ws[n];
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers initialised and tensor memory allocated
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  if (n_units <= n_pairs) pdl_trigger();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+      const uint32_t full0 = mapa_shared(smem_addr(full), 0);
+      const uint64_t keep = l2_evict_last_policy();  // weight tiles: re-read for every token tile
+      int s = 0;
+      uint32_t ph = 0;
+      for (int u = pair; u < n_units; u += n_pairs) {
+        int mt, nt;
+        tile_of(u, mt, nt);
+        const int n0 = nt * 256 + int(rank) * 128, t0 = mt * 256 + int(rank) * 128;
+        for (int kt = 0; kt < nk; ++kt) {
+          mbar_wait(&empty[s], ph ^ 1, FAULT_GEMM_WAIT_EMPTY);
+          const uint32_t fb = full0 + 8u * s;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * SM::STAGE);
+          tma_load_2d_pair_hint(sW + s * SM::OP, &tmW, fb, kt * (I8_BK / 2), n0, keep);
+          tma_load_2d_pair(sX + s * SM::OP, &tmX, fb, kt * (I8_BK / 2), t0);
+          if (++s == SM::STAGES) s = 0, ph ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_i8(256, 256);
+      const uint32_t empty1 = mapa_shared(smem_addr(empty), 1), acc_full1 = mapa_shared(smem_addr(acc_full), 1);
+      int s = 0;
+      uint32_t ph = 0, local = 0;
+      for (int u = pair; u < n_units; u += n_pairs, ++local) {
+        const uint32_t ab = local & 1, aph = (local >> 1) & 1;
+        mbar_wait(&acc_empty[ab], aph ^ 1, FAULT_GEMM_WAIT_ACCUM);
+        tc_fence_after();
+        const uint32_t acc = tmem + ab * 256;
+        for (int kt = 0; kt < nk; ++kt) {
+          mbar_wait(&full[s], ph, FAULT_GEMM_WAIT_FULL_A);
+          tc_fence_after();
+          const uint64_t ad = umma_desc_sw128(smem_addr(sW + s * SM::OP));
+          const uint64_t bd = umma_desc_sw128(smem_addr(sX + s * SM::OP));
+#pragma unroll
+          for (int j = 0; j < I8_BK / 32; ++j)  // 32 bytes of K per MMA = +2 in 16-byte units
+            umma_pair_i8(acc, ad + 2 * j, bd + 2 * j, idesc, (kt != 0 || j != 0) ? 1u : 0u);
+          umma_pair_commit(smem_addr(&empty[s]));  // both CTAs may refill stage s
+          umma_pair_commit(empty1 + 8u * s);
+          if (++s == SM::STAGES) s = 0, ph ^= 1;
+        }
+        umma_pair_commit(smem_addr(&acc_full[ab]));
+        umma_pair_commit(acc_full1 + 8u * ab);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, hf = (warp - 2) >> 2;
+    const uint32_t acc_empty0 = mapa_shared(smem_addr(acc_empty), 0);
+    float* xs = sxs + (warp - 2) * 64;  // token scales of the 64 columns in hand
+    uint32_t local = 0;
+    for (int u = pair; u < n_units; u += n_pairs, ++local) {
+      int mt, nt;
+      tile_of(u, mt, nt);
+      const int n0 = nt * 256 + int(rank) * 128, n = n0 + 32 * q + lane;
+      const int t0 = mt * 256 + 128 * hf;  // this warp's first token
+      const float ws = n < a.n ? a.ws[n] : 0.0f;
+      const uint32_t ab = local & 1, aph = (local >> 1) & 1;
+      const uint32_t tl = tmem + ab * 256 + 128 * hf + (uint32_t(q * 32) << 16);
+      mbar_wait(&acc_full[ab], aph, FAULT_GEMM_WAIT_ACCUM);
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 64) {
+        __syncwarp();
+        xs[lane] = t0 + c + lane < a.m ? a.xs[t0 + c + lane] : 0.0f;
+        xs[lane + 32] = t0 + c + 32 + lane < a.m ? a.xs[t0 + c + 32 + lane] : 0.0f;
+        __syncwarp();
+        if constexpr (EP == B200_EP_SWIGLU) {
+          // Lanes 0..63 of the tile hold gate features, 64..127 the up features of the same
+          // outputs: warps q and q ^ 2 finish 32 of the 64 tokens each and send the other 32.
+          const int side = q >> 1, grp = hf * 2 + (q & 1);
+          float* mine = xch + (grp * 2 + side) * 1024 + lane;
+          const float* theirs = xch + (grp * 2 + (side ^ 1)) * 1024 + lane;
+          const int sc = side ? 0 : 32, oc = side ? 32 : 0;  // columns sent, columns finished
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(tl + c + sc, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mine[32 * j] = i8_value(int(v[j]), xs[sc + j], ws);
+          tmem_ld_32x32b_x32(tl + c + oc, v);
+          tmem_ld_wait();
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + grp) : "memory");
+          const int f = n0 / 2 + 32 * (q & 1) + lane, tt = t0 + c + oc;
+          if (n0 < a.o.n_valid) {
+            size_t idx = size_t(tt) * a.o.ldo + f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j, idx += a.o.ldo) {
+              const float own = i8_value(int(v[j]), xs[oc + j], ws), other = theirs[32 * j];
+              if (tt + j < a.m) store_swiglu(a.o, idx, side ? other : own, side ? own : other);
+            }
+          }
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + grp) : "memory");  // the exchange may be rewritten
+        } else {
+#pragma unroll 1
+          for (int c1 = 0; c1 < 64; c1 += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tl + c + c1, v);
+            tmem_ld_wait();
+            const int tt = t0 + c + c1;
+            if (n < a.o.n_valid) {
+              float* p = static_cast<float*>(a.o.out) + size_t(tt) * a.o.ldo + n;
+              float r[32];
+              if constexpr (EP == B200_EP_RESID_ADD) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = tt + j < a.m ? p[size_t(j) * a.o.ldo] : 0.0f;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float y = i8_value(int(v[j]), xs[c1 + j], ws);
+                if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(r[j], y);
+                if (tt + j < a.m) p[size_t(j) * a.o.ldo] = y;
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * ab);
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA leaves while the other may still read or signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ----------------------------------------------------------------------------- K split over a cluster
+// One CTA = 128 features x bt tokens (a multiple of 16, at most 128) over its share of the K
+// stages; the `split` CTAs of a tile form a cluster. Each turns its int32 sums around in shared
+// memory ([token][feature], where its operands were), and after one cluster barrier CTA r adds the
+// cluster's sums of tokens r * bt / split .. and finishes them. No partial sum reaches global
+// memory and none is added atomically.
+//   warp 0  TMA ring; warp 1  MMAs; then all 8 warps drain the accumulator and finish outputs.
+constexpr int I8S_THREADS = 256;
+constexpr int I8S_OP_W = 128 * I8_BK;
+constexpr int I8S_MAX_STAGES = 12;
+constexpr int I8S_SMEM = 220 * 1024;  // stages
+constexpr int i8s_smem(int stages, int bt) {
+  return 1024 + stages * (I8S_OP_W + bt * I8_BK) + (2 * I8S_MAX_STAGES + 1) * 8 + 16;
+}
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
 }
 
 template <int EP>
-__global__ void gemm_int8_kernel(const I8Args a) {
+__global__ void __launch_bounds__(I8S_THREADS, 1)
+    gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                         const I8Args a) {
+  extern __shared__ uint8_t i8_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
+  const int bt = a.bt, stages = a.stages, split = a.split, x_op = bt * I8_BK;
+  uint8_t* sW = smem;
+  uint8_t* sX = sW + stages * I8S_OP_W;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sX + stages * x_op);
+  uint64_t* empty = full + I8S_MAX_STAGES;
+  uint64_t* acc_full = empty + I8S_MAX_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  int* sP = reinterpret_cast<int*>(smem);  // [bt][128], once the operands are consumed
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % split, n0 = blockIdx.x / split * 128, t0 = blockIdx.y * bt;
+  const int nk = (a.k + I8_BK - 1) / I8_BK;
+  const int kb0 = int(int64_t(rank) * nk / split), kb1 = int(int64_t(rank + 1) * nk / split);
+  const uint32_t cols = bt <= 32 ? 32 : bt <= 64 ? 64 : 128;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+    // weights that lie in HBM start for L2 before the wait for the kernel ahead (a prefetch:
+    // nothing is read that it may still write)
+    for (int kt = kb0; kt < min(kb1, kb0 + 2 * stages); ++kt) tma_prefetch_2d(&tmW, kt * (I8_BK / 2), n0);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  for (int t = blockIdx.y; t < a.m; t += gridDim.y) {
-    if constexpr (EP == B200_EP_SWIGLU) {
-      if (2 * j >= a.o.n_valid) return;
-      const int row = j / 64 * 128 + j % 64;
-      store_swiglu(a.o, t, j, dot_int8(a, t, row), dot_int8(a, t, row + 64));
-    } else {
-      if (j >= a.o.n_valid) return;
-      float* p = static_cast<float*>(a.o.out) + size_t(t) * a.o.ldo + j;
-      const float y = dot_int8(a, t, j);
-      if constexpr (EP == B200_EP_RESID_ADD) *p += y;
-      else *p = y;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kt = kb0; kt < kb1; ++kt) {
+        mbar_wait(&empty[s], ph ^ 1, FAULT_GEMM_WAIT_EMPTY);
+        mbar_arrive_expect_tx(&full[s], I8S_OP_W + x_op);
+        tma_load_2d(sW + s * I8S_OP_W, &tmW, &full[s], kt * (I8_BK / 2), n0);
+        tma_load_2d(sX + s * x_op, &tmX, &full[s], kt * (I8_BK / 2), t0);
+        if (++s == stages) s = 0, ph ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_i8(128, bt);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kt = kb0; kt < kb1; ++kt) {
+        mbar_wait(&full[s], ph, FAULT_GEMM_WAIT_FULL_A);
+        tc_fence_after();
+        const uint64_t ad = umma_desc_sw128(smem_addr(sW + s * I8S_OP_W));
+        const uint64_t bd = umma_desc_sw128(smem_addr(sX + s * x_op));
+#pragma unroll
+        for (int j = 0; j < I8_BK / 32; ++j) umma_i8(tmem, ad + 2 * j, bd + 2 * j, idesc, (kt != kb0 || j != 0) ? 1u : 0u);
+        umma_commit(&empty[s]);
+        if (++s == stages) s = 0, ph ^= 1;
+      }
+      umma_commit(acc_full);
+    }
+    __syncwarp();
+  }
+  mbar_wait(acc_full, 0, FAULT_GEMM_WAIT_ACCUM);
+  tc_fence_after();
+  __syncwarp();
+
+  // ---- sums to shared memory: warp -> lane quarter warp % 4, every second 16 tokens
+  const int q = warp & 3;
+  for (int c = 16 * (warp >> 2); c < bt; c += 32) {
+    uint32_t v[16];
+    tmem_ld_32x32b_x16(tmem + c + (uint32_t(q * 32) << 16), v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sP[(c + j) * 128 + 32 * q + lane] = int(v[j]);
+  }
+  tc_fence_before();
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+
+  // ---- this CTA's tokens: the cluster's sums, scaled and finished
+  const int cnt = bt / split, c0 = rank * cnt;
+  const uint32_t base = smem_addr(sP);
+  uint32_t peer[8];
+#pragma unroll
+  for (int s = 0; s < 8; ++s) peer[s] = s < split ? (split > 1 ? mapa_shared(base, s) : base) : 0;
+  auto total = [&](int col, int l) {
+    const uint32_t off = uint32_t(col * 128 + l) * 4;
+    if (split == 1) return sP[col * 128 + l];
+    int v = 0;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s < split) v += ld_cluster_s32(peer[s] + off);
+    return v;
+  };
+  if constexpr (EP == B200_EP_SWIGLU) {
+    const int l = 32 * (warp & 1) + lane;
+    if (n0 < a.o.n_valid) {
+      const float wg = a.ws[n0 + l], wu = a.ws[n0 + 64 + l];
+#pragma unroll 2
+      for (int c = c0 + (warp >> 1); c < c0 + cnt; c += 4) {
+        const int t = t0 + c;
+        if (t >= a.m) break;
+        const float xs = a.xs[t];
+        store_swiglu(a.o, size_t(t) * a.o.ldo + n0 / 2 + l, i8_value(total(c, l), xs, wg),
+                     i8_value(total(c, l + 64), xs, wu));
+      }
+    }
+  } else {
+    const int l = 32 * q + lane, n = n0 + l;
+    if (n < a.o.n_valid) {
+      const float ws = a.ws[n];
+#pragma unroll 4
+      for (int c = c0 + (warp >> 2); c < c0 + cnt; c += 2) {
+        const int t = t0 + c;
+        if (t >= a.m) break;
+        float* p = static_cast<float*>(a.o.out) + size_t(t) * a.o.ldo + n;
+        float y = i8_value(total(c, l), a.xs[t], ws);
+        if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(*p, y);
+        *p = y;
+      }
+    }
+  }
+  if (split > 1) cluster_sync_all();  // no CTA leaves while its sums may still be read
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
+// ----------------------------------------------------------------------------- at most 16 tokens
+// A matrix-vector product reads each weight once: no ring, barrier or tensor memory before the
+// first MMA. A CTA owns RT 16-feature tiles (the SwiGLU: a gate tile and its up tile) over all of
+// K; its 8 warps take the 64-code k-blocks warp, warp + 8, ... and add their int32 sums through
+// shared memory.
+// Lane (g, t) = (lane / 4, lane % 4) loads codes 16 t .. 16 t + 15 of its k-block of rows g and
+// g + 8 (a quad reads 64 neighbouring bytes), and of tokens g and g + 8. mma.sync m16n8k32 takes 4
+// codes of each row per register: MMA j = 0, 1 is given the words 2 j and 2 j + 1 of both operands,
+// so its k-slots are the same columns on both sides, in an order the sum does not see.
+constexpr int I8R_THREADS = 256;
+constexpr int I8R_WARPS = I8R_THREADS / 32;
+constexpr int I8R_MAX_M = 16;
+constexpr int I8R_DEPTH = 4;  // k-blocks in flight per warp
+
+__device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 weight bytes, read once per call: no L1 allocation
+__device__ __forceinline__ uint4 ld_stream_u4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <int EP, int RT, int NT8>
+__global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Args a) {
+  static_assert(EP != B200_EP_SWIGLU || RT == 2, "a SwiGLU CTA holds a gate tile and its up tile");
+  __shared__ int4 red[I8R_WARPS][RT][NT8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int nkb = (a.k + 63) / 64;
+  int row0[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    if constexpr (EP == B200_EP_SWIGLU) row0[rt] = (blockIdx.x >> 2) * 128 + rt * 64 + (blockIdx.x & 3) * 16;
+    else row0[rt] = (blockIdx.x * RT + rt) * 16;
+  }
+  // weights that lie in HBM start for L2 before the wait for the kernel ahead
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+      if (row0[rt] < a.n) bulk_prefetch_l2(a.w + size_t(row0[rt]) * a.k, uint32_t(min(16, a.n - row0[rt])) * a.k);
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  const int ns = warp < nkb ? (nkb - warp + I8R_WARPS - 1) / I8R_WARPS : 0;
+  uint4 wr[I8R_DEPTH][RT][2], xr[I8R_DEPTH][NT8];
+  int acc[RT][NT8][4] = {};
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  auto load = [&](int d, int s) {
+    const int k0 = (warp + I8R_WARPS * s) * 64 + 16 * t;
+    const bool in = k0 < a.k;  // k is a multiple of 16: a lane's 16 codes are all inside or all outside
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = row0[rt] + g + 8 * h;
+        wr[d][rt][h] = in && row < a.n ? ld_stream_u4(a.w + size_t(row) * a.k + k0) : zero;
+      }
+#pragma unroll
+    for (int i = 0; i < NT8; ++i) {
+      const int tok = 8 * i + g;
+      xr[d][i] = in && tok < a.m ? *reinterpret_cast<const uint4*>(a.q + size_t(tok) * a.ldx + k0) : zero;
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < I8R_DEPTH; ++d)
+    if (d < ns) load(d, d);
+  for (int s0 = 0; s0 < ns; s0 += I8R_DEPTH) {
+#pragma unroll
+    for (int d = 0; d < I8R_DEPTH; ++d) {
+      if (s0 + d < ns) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < NT8; ++i) {
+            const uint4 &u = wr[d][rt][0], &v = wr[d][rt][1], &x = xr[d][i];
+            mma_s8_16832(acc[rt][i], u.x, v.x, u.y, v.y, x.x, x.y);
+            mma_s8_16832(acc[rt][i], u.z, v.z, u.w, v.w, x.z, x.w);
+          }
+        if (s0 + d + I8R_DEPTH < ns) load(d, s0 + d + I8R_DEPTH);
+      }
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int i = 0; i < NT8; ++i)
+      red[warp][rt][i][lane] = make_int4(acc[rt][i][0], acc[rt][i][1], acc[rt][i][2], acc[rt][i][3]);
+  __syncthreads();
+  constexpr int SETS = (EP == B200_EP_SWIGLU ? 1 : RT) * NT8;  // (tile, 8 tokens) finished by a warp each
+  if (warp >= SETS) return;
+  const int rt = warp / NT8, i = warp % NT8;
+  auto sums = [&](int r, int (&v)[4]) {
+    v[0] = v[1] = v[2] = v[3] = 0;
+#pragma unroll
+    for (int w = 0; w < I8R_WARPS; ++w) {
+      const int4 p = red[w][r][i][lane];
+      v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+    }
+  };
+  // lane (g, t) holds row g, tokens 2t and 2t + 1, then row g + 8
+  int v[4];
+  sums(rt, v);
+  if constexpr (EP == B200_EP_SWIGLU) {
+    int u[4];
+    sums(1, u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int tok = 8 * i + 2 * t + (e & 1), l = g + 8 * (e >> 1);
+      if (tok >= a.m) continue;
+      const float xs = a.xs[tok];
+      store_swiglu(a.o, size_t(tok) * a.o.ldo + (blockIdx.x >> 2) * 64 + (blockIdx.x & 3) * 16 + l,
+                   i8_value(v[e], xs, a.ws[row0[0] + l]), i8_value(u[e], xs, a.ws[row0[1] + l]));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int tok = 8 * i + 2 * t + (e & 1), n = row0[rt] + g + 8 * (e >> 1);
+      if (tok >= a.m || n >= a.o.n_valid) continue;
+      float* p = static_cast<float*>(a.o.out) + size_t(tok) * a.o.ldo + n;
+      float y = i8_value(v[e], a.xs[tok], a.ws[n]);
+      if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(*p, y);
+      *p = y;
     }
   }
 }
 
+// ----------------------------------------------------------------------------- host side
+// Codes [rows, k] of ld bytes per row as 128-byte swizzled tiles of 128 codes x box_rows (two
+// codes to a 16-bit element; columns and rows past the end read as zero).
+static int i8_map(CUtensorMap* map, const void* base, int rows, int k, int ld, int box_rows) {
+  const uint64_t dims[2] = {uint64_t(k) / 2, uint64_t(rows)};
+  const uint64_t strides[1] = {uint64_t(ld)};
+  const uint32_t box[2] = {I8_BK / 2, uint32_t(box_rows)};
+  return encode_bf16_sw128(map, base, 2, dims, strides, box);
+}
+
+template <int EP>
+static int launch_i8_pair(I8Args a, cudaStream_t st) {
+  constexpr int smem = I8PairSmem<EP>::TOTAL;
+  static DeviceOnce attr;
+  static int max_pairs_dev[kMaxDevices] = {};  // written under attr's lock, once per device
+  const int r = once_per_device(attr, [](int dev) -> int {
+    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sm_count() & ~1);
+    cfg.blockDim = dim3(I8P_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<EP>, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = sm_count() / 2;
+    }
+    max_pairs_dev[dev] = n;
+    return B200_OK;
+  });
+  if (r != B200_OK) return r;
+  int dev = 0;
+  SDB_CUDA(cudaGetDevice(&dev));
+  CUtensorMap mw, mx;
+  if (int rc = i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
+  if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, 128)) return rc;
+  const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + 255) / 256;
+  // weights beyond what L2 keeps beside the activation stream: groups of about 40 MB
+  const double tile_bytes = 256.0 * a.k;
+  const int groups = n_tiles * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles * tile_bytes / 40e6));
+  a.ngroup = (n_tiles + groups - 1) / groups;
+  const int units = n_tiles * m_tiles;
+  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP>, dim3(2 * std::min(units, max_pairs_dev[dev])), dim3(I8P_THREADS), smem,
+                      st, mw, mx, a));
+  return B200_OK;
+}
+
+template <int EP>
+static int launch_i8_split(I8Args a, cudaStream_t st) {
+  static DeviceOnce attr;
+  const int r = once_per_device(attr, [](int) -> int {
+    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    return B200_OK;
+  });
+  if (r != B200_OK) return r;
+  const int nk = (a.k + I8_BK - 1) / I8_BK, n_tiles = (a.o.n_valid + 127) / 128;
+  int m_tiles = (a.m + 127) / 128;
+  a.bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
+  m_tiles = (a.m + a.bt - 1) / a.bt;
+  const int tiles = n_tiles * m_tiles;
+  a.split = 1;
+  while (a.split < 8 && 2 * a.split * tiles <= sm_count() && 4 * a.split <= nk) a.split *= 2;
+  const int stage = I8S_OP_W + a.bt * I8_BK;
+  a.stages = std::min({I8S_MAX_STAGES, I8S_SMEM / stage, std::max(4, (nk + a.split - 1) / a.split)});
+  CUtensorMap mw, mx;
+  if (int rc = i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
+  if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, a.bt)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.split * n_tiles, m_tiles);
+  cfg.blockDim = dim3(I8S_THREADS);
+  cfg.dynamicSmemBytes = i8s_smem(a.stages, a.bt);
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = a.split;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  SDB_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<EP>, mw, mx, a));
+  return B200_OK;
+}
+
+template <int EP, int RT, int NT8>
+static int launch_i8_reg(const I8Args& a, cudaStream_t st) {
+  const int grid = (a.o.n_valid + 16 * RT - 1) / (16 * RT);
+  SDB_CUDA(launch_pdl(gemm_i8_reg_kernel<EP, RT, NT8>, dim3(grid), dim3(I8R_THREADS), 0, st, a));
+  return B200_OK;
+}
+
 template <int EP>
 static int launch_int8(const I8Args& a, cudaStream_t st) {
-  const int cols = EP == B200_EP_SWIGLU ? a.o.n_valid / 2 : a.o.n_valid;
-  SDB_CUDA(launch_pdl(gemm_int8_kernel<EP>, dim3((cols + 127) / 128, std::min(a.m, 65535)), dim3(128), 0, st, a));
-  return B200_OK;
+  constexpr int RT = EP == B200_EP_SWIGLU ? 2 : 1;
+  if (a.m <= 8) return launch_i8_reg<EP, RT, 1>(a, st);
+  if (a.m <= I8R_MAX_M) return launch_i8_reg<EP, RT, 2>(a, st);
+  // pairs once every pair has a whole tile
+  const int64_t units = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
+  return units >= sm_count() / 2 ? launch_i8_pair<EP>(a, st) : launch_i8_split<EP>(a, st);
 }
 
 int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
@@ -95,7 +716,7 @@ int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k,
     return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: out is not aligned to its elements");
   if (out->lo_format != B200_LO_BF16 && out->lo_format != B200_LO_E4M3)
     return sdb_fail(B200_ERR_ARG, "b200_linear_int8: unknown lo_format");
-  I8Args a{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx};
+  I8Args a{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx, 1, 0, 0, 1};
   switch (out->epilogue) {
     case B200_EP_STORE: return launch_int8<B200_EP_STORE>(a, st);
     case B200_EP_RESID_ADD: return launch_int8<B200_EP_RESID_ADD>(a, st);
