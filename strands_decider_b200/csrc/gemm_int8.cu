@@ -35,18 +35,20 @@ __device__ __forceinline__ float i8_value(int acc, float xs, float ws) {
   return __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws);
 }
 
-// The SwiGLU's output at element idx of the planes: silu(g) * u as the bf16 hi plane and, if
-// asked, the low plane.
+// The SwiGLU's output at element idx of the planes: silu(g) * u as the bf16 hi plane and, with LO,
+// the low plane.
+template <bool LO>
 __device__ __forceinline__ void store_swiglu(const b200_linear_out& o, size_t idx, float g, float u) {
   const float h = __fmul_rn(silu_approx(g), u);
   const uint16_t hb = f32_to_bf16_rn(h);
   uint16_t* dst = static_cast<uint16_t*>(o.out);
   dst[idx] = hb;
-  if (!o.lo_offset) return;
-  if (o.lo_format == B200_LO_E4M3)
-    reinterpret_cast<uint8_t*>(dst + o.lo_offset)[idx] = uint8_t(f32x2_to_e4m3x2(lo8_value(h, hb), 0.0f));
-  else
-    dst[o.lo_offset + idx] = f32_to_bf16_rn(h - bf16_to_f32(hb));
+  if constexpr (LO) {
+    if (o.lo_format == B200_LO_E4M3)
+      reinterpret_cast<uint8_t*>(dst + o.lo_offset)[idx] = uint8_t(f32x2_to_e4m3x2(lo8_value(h, hb), 0.0f));
+    else
+      dst[o.lo_offset + idx] = f32_to_bf16_rn(h - bf16_to_f32(hb));
+  }
 }
 
 // Instruction descriptor, kind::i8: D s32, A and B signed bytes, both K-major, M x N.
@@ -76,6 +78,28 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
+// Waits for this warp's tcgen05.ld's; the registers they fill pass through, so that nothing that
+// uses them moves ahead of the wait.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                 "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                 "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
                "r"(x), "r"(y)
@@ -88,23 +112,45 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, i
 //   warp 0      TMA ring (both CTAs; bytes signalled on the leader's full barrier)
 //   warp 1      the leader's lane 0 issues the MMAs into one of two 256-column accumulators
 //   warps 2..9  epilogue: TMEM lane quarter warp % 4, token half (warp - 2) / 4
+//               (128 tokens, 32 at a time; the next ones leave TMEM while these are finished)
 constexpr int I8P_THREADS = 320;
 constexpr int I8P_EPI_WARPS = 8;
+constexpr int I8P_XCH_LD = 20;  // floats per lane of an exchange buffer (16 tokens; 16-byte accesses
+                                // of 8 neighbouring lanes then fall into different banks)
 
 template <int EP>
 struct I8PairSmem {
   static constexpr int OP = 128 * I8_BK;                    // one operand of a stage
   static constexpr int STAGE = 2 * OP;
-  // the SwiGLU gives one stage for the exchange of gate and up sums between lane halves
+  // the SwiGLU gives one stage for the exchange of gate and up sums between lane halves:
+  // [round parity][token half, feature half][side][lane][16 tokens]
   static constexpr int STAGES = EP == B200_EP_SWIGLU ? 5 : 6;
-  static constexpr int XCH = EP == B200_EP_SWIGLU ? 4 * 2 * 32 * 32 * 4 : 0;
-  static constexpr int XS = I8P_EPI_WARPS * 64 * 4;         // each epilogue warp's token scales
+  static constexpr int XCH = EP == B200_EP_SWIGLU ? 2 * 4 * 2 * 32 * I8P_XCH_LD * 4 : 0;
+  static constexpr int XS = I8P_EPI_WARPS * 128 * 4;        // each epilogue warp's token scales
   static constexpr int BARS = 2 * STAGES + 4;
   static constexpr int TOTAL = 1024 + STAGES * STAGE + XCH + XS + BARS * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
-template <int EP>
+// CW neighbouring columns (tokens) of one accumulator lane (feature), stored at p and ldo apart.
+// FULL: all of them are inside the batch.
+template <int EP, bool FULL, int CW>
+__device__ __forceinline__ void i8_finish(const I8Args& a, const uint32_t (&v)[CW], const float* xs, float ws, float* p,
+                                          const float (&r)[CW], int left) {
+#pragma unroll
+  for (int j = 0; j < CW; j += 4) {
+    const float4 x4 = *reinterpret_cast<const float4*>(xs + j);
+    const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float y = i8_value(int(v[j + e]), x[e], ws);
+      if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(r[j + e], y);
+      if (FULL || j + e < left) p[size_t(j + e) * a.o.ldo] = y;
+    }
+  }
+}
+
+template <int EP, bool LO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                         const I8Args a) {
@@ -213,71 +259,104 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   } else {
     const int q = warp & 3, hf = (warp - 2) >> 2;
     const uint32_t acc_empty0 = mapa_shared(smem_addr(acc_empty), 0);
-    float* xs = sxs + (warp - 2) * 64;  // token scales of the 64 columns in hand
+    float* xs = sxs + (warp - 2) * 128;  // scales of this warp's 128 tokens
     uint32_t local = 0;
     for (int u = pair; u < n_units; u += n_pairs, ++local) {
       int mt, nt;
       tile_of(u, mt, nt);
       const int n0 = nt * 256 + int(rank) * 128, n = n0 + 32 * q + lane;
-      const int t0 = mt * 256 + 128 * hf;  // this warp's first token
+      const int t0 = mt * 256 + 128 * hf, left = a.m - t0;  // this warp's first token, tokens from it on
       const float ws = n < a.n ? a.ws[n] : 0.0f;
       const uint32_t ab = local & 1, aph = (local >> 1) & 1;
       const uint32_t tl = tmem + ab * 256 + 128 * hf + (uint32_t(q * 32) << 16);
-      mbar_wait(&acc_full[ab], aph, FAULT_GEMM_WAIT_ACCUM);
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < 128; c += 64) {
-        __syncwarp();
-        xs[lane] = t0 + c + lane < a.m ? a.xs[t0 + c + lane] : 0.0f;
-        xs[lane + 32] = t0 + c + 32 + lane < a.m ? a.xs[t0 + c + 32 + lane] : 0.0f;
-        __syncwarp();
-        if constexpr (EP == B200_EP_SWIGLU) {
-          // Lanes 0..63 of the tile hold gate features, 64..127 the up features of the same
-          // outputs: warps q and q ^ 2 finish 32 of the 64 tokens each and send the other 32.
-          const int side = q >> 1, grp = hf * 2 + (q & 1);
-          float* mine = xch + (grp * 2 + side) * 1024 + lane;
-          const float* theirs = xch + (grp * 2 + (side ^ 1)) * 1024 + lane;
-          const int sc = side ? 0 : 32, oc = side ? 32 : 0;  // columns sent, columns finished
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(tl + c + sc, v);
-          tmem_ld_wait();
+      float xv[4];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) mine[32 * j] = i8_value(int(v[j]), xs[sc + j], ws);
-          tmem_ld_32x32b_x32(tl + c + oc, v);
-          tmem_ld_wait();
+      for (int i = 0; i < 4; ++i) xv[i] = 32 * i + lane < left ? a.xs[t0 + 32 * i + lane] : 0.0f;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xs[32 * i + lane] = xv[i];
+      __syncwarp();
+      if constexpr (EP == B200_EP_SWIGLU) {
+        // Lanes 0..63 of the tile hold gate features, 64..127 the up features of the same outputs:
+        // of every 32 tokens warps q and q ^ 2 finish 16 each and send the other 16. Two buffers by
+        // round parity: a warp reaches a round's barrier only after it has read the round before.
+        const int side = q >> 1, grp = hf * 2 + (q & 1);
+        const int sc = side ? 0 : 16, oc = side ? 16 : 0;  // columns sent, columns finished
+        float* mine = xch + ((grp * 2 + side) * 32 + lane) * I8P_XCH_LD;
+        const float* theirs = xch + ((grp * 2 + (side ^ 1)) * 32 + lane) * I8P_XCH_LD;
+        constexpr int XB = 4 * 2 * 32 * I8P_XCH_LD;  // floats of one parity's buffers
+        const bool valid = n0 < a.o.n_valid;
+        const size_t idx0 = size_t(t0 + oc) * a.o.ldo + n0 / 2 + 32 * (q & 1) + lane;
+        uint32_t vs[2][16], vo[2][16];
+        mbar_wait(&acc_full[ab], aph, FAULT_GEMM_WAIT_ACCUM);
+        tc_fence_after();
+        tmem_ld(tl + sc, vs[0]);
+        tmem_ld(tl + oc, vo[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait_for(vs[c & 1]);
+          tmem_ld_wait_for(vo[c & 1]);
+          if (c < 3) {
+            tmem_ld(tl + 32 * (c + 1) + sc, vs[(c + 1) & 1]);
+            tmem_ld(tl + 32 * (c + 1) + oc, vo[(c + 1) & 1]);
+          }
+          const float* xc = xs + 32 * c;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(xc + sc + j);
+            *reinterpret_cast<float4*>(mine + (c & 1) * XB + j) =
+                make_float4(i8_value(int(vs[c & 1][j]), x.x, ws), i8_value(int(vs[c & 1][j + 1]), x.y, ws),
+                            i8_value(int(vs[c & 1][j + 2]), x.z, ws), i8_value(int(vs[c & 1][j + 3]), x.w, ws));
+          }
           asm volatile("bar.sync %0, 64;" ::"r"(1 + grp) : "memory");
-          const int f = n0 / 2 + 32 * (q & 1) + lane, tt = t0 + c + oc;
-          if (n0 < a.o.n_valid) {
-            size_t idx = size_t(tt) * a.o.ldo + f;
+          if (valid) {
+            const int l = left - 32 * c - oc;  // of these 16 tokens, the ones inside the batch
+            const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
 #pragma unroll
-            for (int j = 0; j < 32; ++j, idx += a.o.ldo) {
-              const float own = i8_value(int(v[j]), xs[oc + j], ws), other = theirs[32 * j];
-              if (tt + j < a.m) store_swiglu(a.o, idx, side ? other : own, side ? own : other);
-            }
-          }
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + grp) : "memory");  // the exchange may be rewritten
-        } else {
-#pragma unroll 1
-          for (int c1 = 0; c1 < 64; c1 += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(tl + c + c1, v);
-            tmem_ld_wait();
-            const int tt = t0 + c + c1;
-            if (n < a.o.n_valid) {
-              float* p = static_cast<float*>(a.o.out) + size_t(tt) * a.o.ldo + n;
-              float r[32];
-              if constexpr (EP == B200_EP_RESID_ADD) {
+            for (int j = 0; j < 16; j += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(xc + oc + j);
+              const float4 o4 = *reinterpret_cast<const float4*>(theirs + (c & 1) * XB + j);
+              const float xe[4] = {x.x, x.y, x.z, x.w}, oe[4] = {o4.x, o4.y, o4.z, o4.w};
 #pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = tt + j < a.m ? p[size_t(j) * a.o.ldo] : 0.0f;
-              }
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float y = i8_value(int(v[j]), xs[c1 + j], ws);
-                if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(r[j], y);
-                if (tt + j < a.m) p[size_t(j) * a.o.ldo] = y;
+              for (int e = 0; e < 4; ++e) {
+                const float own = i8_value(int(vo[c & 1][j + e]), xe[e], ws);
+                if (j + e < l)
+                  store_swiglu<LO>(a.o, idx + size_t(j + e) * a.o.ldo, side ? oe[e] : own, side ? own : oe[e]);
               }
             }
           }
+        }
+      } else {
+        float* p = static_cast<float*>(a.o.out) + size_t(t0) * a.o.ldo + n;
+        const bool valid = n < a.o.n_valid;
+        constexpr int CW = EP == B200_EP_RESID_ADD ? 16 : 32;  // columns in hand (and as many ahead)
+        float r[2][CW];
+        auto residual = [&](int c) {  // chunk c's residual, read while the chunk before is finished
+          if constexpr (EP == B200_EP_RESID_ADD) {
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+              r[c & 1][j] = valid && CW * c + j < left ? p[size_t(CW * c + j) * a.o.ldo] : 0.0f;
+          }
+        };
+        residual(0);
+        uint32_t v[2][CW];
+        mbar_wait(&acc_full[ab], aph, FAULT_GEMM_WAIT_ACCUM);
+        tc_fence_after();
+        tmem_ld(tl, v[0]);
+#pragma unroll
+        for (int c = 0; c < 128 / CW; ++c) {
+          tmem_ld_wait_for(v[c & 1]);
+          if (c + 1 < 128 / CW) {
+            tmem_ld(tl + CW * (c + 1), v[(c + 1) & 1]);
+            residual(c + 1);
+          }
+          if (valid) {
+            float* pc = p + size_t(CW * c) * a.o.ldo;
+            const int l = left - CW * c;
+            if (l >= CW) i8_finish<EP, true>(a, v[c & 1], xs + CW * c, ws, pc, r[c & 1], l);
+            else i8_finish<EP, false>(a, v[c & 1], xs + CW * c, ws, pc, r[c & 1], l);
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -306,7 +385,7 @@ constexpr int I8S_OP_W = 128 * I8_BK;
 constexpr int I8S_MAX_STAGES = 12;
 constexpr int I8S_SMEM = 220 * 1024;  // stages
 constexpr int i8s_smem(int stages, int bt) {
-  return 1024 + stages * (I8S_OP_W + bt * I8_BK) + (2 * I8S_MAX_STAGES + 1) * 8 + 16;
+  return 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (2 * I8S_MAX_STAGES + 1) * 8 + 16;
 }
 
 __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
@@ -315,7 +394,7 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   return v;
 }
 
-template <int EP>
+template <int EP, bool LO>
 __global__ void __launch_bounds__(I8S_THREADS, 1)
     gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                          const I8Args a) {
@@ -324,7 +403,8 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
   const int bt = a.bt, stages = a.stages, split = a.split, x_op = bt * I8_BK;
   uint8_t* sW = smem;
   uint8_t* sX = sW + stages * I8S_OP_W;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sX + stages * x_op);
+  float* sxs = reinterpret_cast<float*>(sX + stages * x_op);  // [bt] token scales
+  uint64_t* full = reinterpret_cast<uint64_t*>(sxs + 128);
   uint64_t* empty = full + I8S_MAX_STAGES;
   uint64_t* acc_full = empty + I8S_MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
@@ -357,6 +437,8 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();
+  if (threadIdx.x >= 128 && int(threadIdx.x) - 128 < bt)
+    sxs[threadIdx.x - 128] = t0 + int(threadIdx.x) - 128 < a.m ? a.xs[t0 + threadIdx.x - 128] : 0.0f;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -398,8 +480,8 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
   const int q = warp & 3;
   for (int c = 16 * (warp >> 2); c < bt; c += 32) {
     uint32_t v[16];
-    tmem_ld_32x32b_x16(tmem + c + (uint32_t(q * 32) << 16), v);
-    tmem_ld_wait();
+    tmem_ld(tmem + c + (uint32_t(q * 32) << 16), v);
+    tmem_ld_wait_for(v);
 #pragma unroll
     for (int j = 0; j < 16; ++j) sP[(c + j) * 128 + 32 * q + lane] = int(v[j]);
   }
@@ -407,12 +489,14 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
   if (split > 1) cluster_sync_all();
   else __syncthreads();
 
-  // ---- this CTA's tokens: the cluster's sums, scaled and finished
+  // ---- this CTA's tokens: the cluster's sums, scaled and finished; every load of a batch of
+  // tokens (sums, residual) is issued before its first store
   const int cnt = bt / split, c0 = rank * cnt;
+  const int c_end = min(c0 + cnt, a.m - t0);
   const uint32_t base = smem_addr(sP);
   uint32_t peer[8];
 #pragma unroll
-  for (int s = 0; s < 8; ++s) peer[s] = s < split ? (split > 1 ? mapa_shared(base, s) : base) : 0;
+  for (int s = 0; s < 8; ++s) peer[s] = s < split && split > 1 ? mapa_shared(base, s) : base;
   auto total = [&](int col, int l) {
     const uint32_t off = uint32_t(col * 128 + l) * 4;
     if (split == 1) return sP[col * 128 + l];
@@ -422,31 +506,51 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
       if (s < split) v += ld_cluster_s32(peer[s] + off);
     return v;
   };
+  constexpr int TB = 8;  // tokens per batch
   if constexpr (EP == B200_EP_SWIGLU) {
     const int l = 32 * (warp & 1) + lane;
     if (n0 < a.o.n_valid) {
       const float wg = a.ws[n0 + l], wu = a.ws[n0 + 64 + l];
-#pragma unroll 2
-      for (int c = c0 + (warp >> 1); c < c0 + cnt; c += 4) {
-        const int t = t0 + c;
-        if (t >= a.m) break;
-        const float xs = a.xs[t];
-        store_swiglu(a.o, size_t(t) * a.o.ldo + n0 / 2 + l, i8_value(total(c, l), xs, wg),
-                     i8_value(total(c, l + 64), xs, wu));
+      for (int cb = c0 + (warp >> 1); cb < c_end; cb += 4 * TB) {
+        int g[TB], u[TB];
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+          const int c = min(cb + 4 * i, c_end - 1);
+          g[i] = total(c, l);
+          u[i] = total(c, l + 64);
+        }
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+          const int c = cb + 4 * i;
+          if (c < c_end)
+            store_swiglu<LO>(a.o, size_t(t0 + c) * a.o.ldo + n0 / 2 + l, i8_value(g[i], sxs[c], wg),
+                             i8_value(u[i], sxs[c], wu));
+        }
       }
     }
   } else {
     const int l = 32 * q + lane, n = n0 + l;
     if (n < a.o.n_valid) {
       const float ws = a.ws[n];
-#pragma unroll 4
-      for (int c = c0 + (warp >> 2); c < c0 + cnt; c += 2) {
-        const int t = t0 + c;
-        if (t >= a.m) break;
-        float* p = static_cast<float*>(a.o.out) + size_t(t) * a.o.ldo + n;
-        float y = i8_value(total(c, l), a.xs[t], ws);
-        if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(*p, y);
-        *p = y;
+      float* out = static_cast<float*>(a.o.out) + n;
+      for (int cb = c0 + (warp >> 2); cb < c_end; cb += 2 * TB) {
+        int v[TB];
+        float r[TB];
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+          const int c = min(cb + 2 * i, c_end - 1);
+          v[i] = total(c, l);
+          if constexpr (EP == B200_EP_RESID_ADD) r[i] = out[size_t(t0 + c) * a.o.ldo];
+        }
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+          const int c = cb + 2 * i;
+          if (c < c_end) {
+            float y = i8_value(v[i], sxs[c], ws);
+            if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(r[i], y);
+            out[size_t(t0 + c) * a.o.ldo] = y;
+          }
+        }
       }
     }
   }
@@ -576,8 +680,10 @@ __global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Arg
       const int tok = 8 * i + 2 * t + (e & 1), l = g + 8 * (e >> 1);
       if (tok >= a.m) continue;
       const float xs = a.xs[tok];
-      store_swiglu(a.o, size_t(tok) * a.o.ldo + (blockIdx.x >> 2) * 64 + (blockIdx.x & 3) * 16 + l,
-                   i8_value(v[e], xs, a.ws[row0[0] + l]), i8_value(u[e], xs, a.ws[row0[1] + l]));
+      const float g = i8_value(v[e], xs, a.ws[row0[0] + l]), up = i8_value(u[e], xs, a.ws[row0[1] + l]);
+      const size_t idx = size_t(tok) * a.o.ldo + (blockIdx.x >> 2) * 64 + (blockIdx.x & 3) * 16 + l;
+      if (a.o.lo_offset) store_swiglu<true>(a.o, idx, g, up);
+      else store_swiglu<false>(a.o, idx, g, up);
     }
   } else {
 #pragma unroll
@@ -602,19 +708,19 @@ static int i8_map(CUtensorMap* map, const void* base, int rows, int k, int ld, i
   return encode_bf16_sw128(map, base, 2, dims, strides, box);
 }
 
-template <int EP>
+template <int EP, bool LO>
 static int launch_i8_pair(I8Args a, cudaStream_t st) {
   constexpr int smem = I8PairSmem<EP>::TOTAL;
   static DeviceOnce attr;
   static int max_pairs_dev[kMaxDevices] = {};  // written under attr's lock, once per device
   const int r = once_per_device(attr, [](int dev) -> int {
-    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<EP, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sm_count() & ~1);
     cfg.blockDim = dim3(I8P_THREADS);
     cfg.dynamicSmemBytes = smem;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<EP>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<EP, LO>, &cfg) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = sm_count() / 2;
     }
@@ -633,16 +739,16 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   const int groups = n_tiles * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles * tile_bytes / 40e6));
   a.ngroup = (n_tiles + groups - 1) / groups;
   const int units = n_tiles * m_tiles;
-  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP>, dim3(2 * std::min(units, max_pairs_dev[dev])), dim3(I8P_THREADS), smem,
+  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP, LO>, dim3(2 * std::min(units, max_pairs_dev[dev])), dim3(I8P_THREADS), smem,
                       st, mw, mx, a));
   return B200_OK;
 }
 
-template <int EP>
+template <int EP, bool LO>
 static int launch_i8_split(I8Args a, cudaStream_t st) {
   static DeviceOnce attr;
   const int r = once_per_device(attr, [](int) -> int {
-    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<EP, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     return B200_OK;
   });
   if (r != B200_OK) return r;
@@ -671,7 +777,7 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  SDB_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<EP>, mw, mx, a));
+  SDB_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<EP, LO>, mw, mx, a));
   return B200_OK;
 }
 
@@ -689,7 +795,11 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   if (a.m <= I8R_MAX_M) return launch_i8_reg<EP, RT, 2>(a, st);
   // pairs once every pair has a whole tile
   const int64_t units = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
-  return units >= sm_count() / 2 ? launch_i8_pair<EP>(a, st) : launch_i8_split<EP>(a, st);
+  const bool pairs = units >= sm_count() / 2;
+  if constexpr (EP == B200_EP_SWIGLU) {
+    if (a.o.lo_offset) return pairs ? launch_i8_pair<EP, true>(a, st) : launch_i8_split<EP, true>(a, st);
+  }
+  return pairs ? launch_i8_pair<EP, false>(a, st) : launch_i8_split<EP, false>(a, st);
 }
 
 int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
