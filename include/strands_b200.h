@@ -208,7 +208,7 @@ int b200_quantize_act_int8(const void* x, const uint16_t* x_lo, int32_t type, in
  * x fp32 [rows, ldx]; delta (optional) fp32 or bf16 [rows, ldd]; sum (optional, needs delta)
  * receives t as fp32 [rows, lds] and may be x or an fp32 delta themselves (same stride), with no
  * other overlap. hidden a multiple of 16, at most 65536; every row stride in bytes a multiple of
- * 16 and every pointer 16-byte aligned; eps >= 0. */
+ * 16 and every pointer 16-byte aligned; eps > 0. */
 int b200_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd, float* sum,
                       int32_t lds, int32_t rows, int32_t hidden, const float* w, float eps, int8_t* q, int32_t ldq,
                       float* scale, b200_stream stream);

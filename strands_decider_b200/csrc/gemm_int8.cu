@@ -26,7 +26,8 @@ struct I8Args {
   b200_linear_out o;
   int m, n, k, ldx;
   int ngroup;           // pair kernel: feature tiles per group
-  int bt, stages, split;  // split kernel: tokens per tile, ring depth, CTAs per tile
+  int bt, stages;       // split kernel: tokens per tile, ring depth
+  int vec;              // output rows take 16-byte (SwiGLU: 8-byte) accesses at every fourth output
 };
 
 constexpr int I8_BK = 128;  // bytes (= codes) of K per stage: one 128-byte swizzled row
@@ -35,11 +36,19 @@ __device__ __forceinline__ float i8_value(int acc, float xs, float ws) {
   return __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws);
 }
 
+// silu(g) u = g u / (1 + 2^(-g log2 e)), flushing what underflows: 2^x to 0 where 1 + 2^x is 1
+// anyway, 1 / (1 + 2^x) to 0 from 2^126 on, where the quotient is below 2^-119 (a NaN stays one).
+__device__ __forceinline__ float swiglu(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(g, -1.4426950408889634f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return __fmul_rn(__fmul_rn(g, r), u);
+}
 // The SwiGLU's output at element idx of the planes: silu(g) * u as the bf16 hi plane and, with LO,
 // the low plane.
 template <bool LO>
 __device__ __forceinline__ void store_swiglu(const b200_linear_out& o, size_t idx, float g, float u) {
-  const float h = __fmul_rn(silu_approx(g), u);
+  const float h = swiglu(g, u);
   const uint16_t hb = f32_to_bf16_rn(h);
   uint16_t* dst = static_cast<uint16_t*>(o.out);
   dst[idx] = hb;
@@ -375,32 +384,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 
 // ----------------------------------------------------------------------------- K split over a cluster
 // One CTA = 128 features x bt tokens (a multiple of 16, at most 128) over its share of the K
-// stages; the `split` CTAs of a tile form a cluster. Each turns its int32 sums around in shared
+// stages; the SPLIT CTAs of a tile form a cluster. Each turns its int32 sums around in shared
 // memory ([token][feature], where its operands were), and after one cluster barrier CTA r adds the
-// cluster's sums of tokens r * bt / split .. and finishes them. No partial sum reaches global
+// cluster's sums of tokens r * bt / SPLIT .. and finishes them. No partial sum reaches global
 // memory and none is added atomically.
 //   warp 0  TMA ring; warp 1  MMAs; then all 8 warps drain the accumulator and finish outputs.
 constexpr int I8S_THREADS = 256;
 constexpr int I8S_OP_W = 128 * I8_BK;
 constexpr int I8S_MAX_STAGES = 12;
-constexpr int I8S_SMEM = 220 * 1024;  // stages
+constexpr int I8S_RING = 220 * 1024;       // bytes of stages: one CTA per SM
+constexpr int I8S_RING_HALF = 104 * 1024;  // two CTAs per SM
 constexpr int i8s_smem(int stages, int bt) {
   return 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (2 * I8S_MAX_STAGES + 1) * 8 + 16;
 }
 
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
+__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
   return v;
 }
+__device__ __forceinline__ int4 add4(int4 a, int4 b) { return make_int4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
-template <int EP, bool LO>
+template <int EP, bool LO, int SPLIT>
 __global__ void __launch_bounds__(I8S_THREADS, 1)
     gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                          const I8Args a) {
   extern __shared__ uint8_t i8_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
-  const int bt = a.bt, stages = a.stages, split = a.split, x_op = bt * I8_BK;
+  const int bt = a.bt, stages = a.stages, x_op = bt * I8_BK;
   uint8_t* sW = smem;
   uint8_t* sX = sW + stages * I8S_OP_W;
   float* sxs = reinterpret_cast<float*>(sX + stages * x_op);  // [bt] token scales
@@ -411,9 +424,9 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
   int* sP = reinterpret_cast<int*>(smem);  // [bt][128], once the operands are consumed
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % split, n0 = blockIdx.x / split * 128, t0 = blockIdx.y * bt;
+  const int rank = blockIdx.x % SPLIT, n0 = blockIdx.x / SPLIT * 128, t0 = blockIdx.y * bt;
   const int nk = (a.k + I8_BK - 1) / I8_BK;
-  const int kb0 = int(int64_t(rank) * nk / split), kb1 = int(int64_t(rank + 1) * nk / split);
+  const int kb0 = int(int64_t(rank) * nk / SPLIT), kb1 = int(int64_t(rank + 1) * nk / SPLIT);
   const uint32_t cols = bt <= 32 ? 32 : bt <= 64 ? 64 : 128;
 
   if (threadIdx.x == 0) {
@@ -472,6 +485,38 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
     }
     __syncwarp();
   }
+
+  // what the outputs need besides the sums, read while the sums are formed: the channel scales of
+  // this lane's four features, and the residual of the warp's first TB tokens
+  const int cnt = bt / SPLIT, c0 = rank * cnt;
+  const int c_end = min(c0 + cnt, a.m - t0);
+  const int f = n0 + 4 * lane;
+  constexpr int TB = SPLIT == 8 ? 2 : 4;  // tokens per batch: its loads are all issued before its first store
+  float ws[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ws[e] = f + e < a.n ? a.ws[f + e] : 0.0f;
+  float4 r[TB];
+  auto residual = [&](int cb) {
+    if constexpr (EP == B200_EP_RESID_ADD) {
+#pragma unroll
+      for (int i = 0; i < TB; ++i) {
+        const int c = cb + 8 * i;
+        const float* p = static_cast<const float*>(a.o.out) + size_t(t0 + c) * a.o.ldo + f;
+        r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < c_end && f < a.o.n_valid) {
+          if (a.vec && f + 4 <= a.o.n_valid) {
+            r[i] = *reinterpret_cast<const float4*>(p);
+          } else {
+            r[i].x = p[0];
+            if (f + 1 < a.o.n_valid) r[i].y = p[1];
+            if (f + 2 < a.o.n_valid) r[i].z = p[2];
+            if (f + 3 < a.o.n_valid) r[i].w = p[3];
+          }
+        }
+      }
+    }
+  };
+  residual(c0 + warp);
   mbar_wait(acc_full, 0, FAULT_GEMM_WAIT_ACCUM);
   tc_fence_after();
   __syncwarp();
@@ -486,75 +531,73 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
     for (int j = 0; j < 16; ++j) sP[(c + j) * 128 + 32 * q + lane] = int(v[j]);
   }
   tc_fence_before();
-  if (split > 1) cluster_sync_all();
+  if (SPLIT > 1) cluster_sync_all();
   else __syncthreads();
 
-  // ---- this CTA's tokens: the cluster's sums, scaled and finished; every load of a batch of
-  // tokens (sums, residual) is issued before its first store
-  const int cnt = bt / split, c0 = rank * cnt;
-  const int c_end = min(c0 + cnt, a.m - t0);
+  // ---- this CTA's tokens: the cluster's sums, scaled and finished. A warp takes whole tokens,
+  // four features per lane: 16-byte reads of each CTA's sums (4-byte ones through distributed
+  // shared memory took the most of the kernel) and 16-byte stores where the output is aligned.
   const uint32_t base = smem_addr(sP);
-  uint32_t peer[8];
+  for (int cb = c0 + warp; cb < c_end; cb += 8 * TB) {
+    if (cb != c0 + warp) residual(cb);
+    int4 v[TB], part[TB][SPLIT];
 #pragma unroll
-  for (int s = 0; s < 8; ++s) peer[s] = s < split && split > 1 ? mapa_shared(base, s) : base;
-  auto total = [&](int col, int l) {
-    const uint32_t off = uint32_t(col * 128 + l) * 4;
-    if (split == 1) return sP[col * 128 + l];
-    int v = 0;
+    for (int i = 0; i < TB; ++i) {
+      const int c = min(cb + 8 * i, c_end - 1);
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      if (s < split) v += ld_cluster_s32(peer[s] + off);
-    return v;
-  };
-  constexpr int TB = 8;  // tokens per batch
-  if constexpr (EP == B200_EP_SWIGLU) {
-    const int l = 32 * (warp & 1) + lane;
-    if (n0 < a.o.n_valid) {
-      const float wg = a.ws[n0 + l], wu = a.ws[n0 + 64 + l];
-      for (int cb = c0 + (warp >> 1); cb < c_end; cb += 4 * TB) {
-        int g[TB], u[TB];
-#pragma unroll
-        for (int i = 0; i < TB; ++i) {
-          const int c = min(cb + 4 * i, c_end - 1);
-          g[i] = total(c, l);
-          u[i] = total(c, l + 64);
-        }
-#pragma unroll
-        for (int i = 0; i < TB; ++i) {
-          const int c = cb + 4 * i;
-          if (c < c_end)
-            store_swiglu<LO>(a.o, size_t(t0 + c) * a.o.ldo + n0 / 2 + l, i8_value(g[i], sxs[c], wg),
-                             i8_value(u[i], sxs[c], wu));
-        }
+      for (int s = 0; s < SPLIT; ++s) {
+        if constexpr (SPLIT == 1) part[i][s] = *reinterpret_cast<const int4*>(sP + c * 128 + 4 * lane);
+        else part[i][s] = ld_cluster_s32x4(mapa_shared(base + uint32_t(c * 128 + 4 * lane) * 4, s));
       }
     }
-  } else {
-    const int l = 32 * q + lane, n = n0 + l;
-    if (n < a.o.n_valid) {
-      const float ws = a.ws[n];
-      float* out = static_cast<float*>(a.o.out) + n;
-      for (int cb = c0 + (warp >> 2); cb < c_end; cb += 2 * TB) {
-        int v[TB];
-        float r[TB];
 #pragma unroll
-        for (int i = 0; i < TB; ++i) {
-          const int c = min(cb + 2 * i, c_end - 1);
-          v[i] = total(c, l);
-          if constexpr (EP == B200_EP_RESID_ADD) r[i] = out[size_t(t0 + c) * a.o.ldo];
-        }
+    for (int i = 0; i < TB; ++i) {
+      v[i] = part[i][0];
 #pragma unroll
-        for (int i = 0; i < TB; ++i) {
-          const int c = cb + 2 * i;
-          if (c < c_end) {
-            float y = i8_value(v[i], sxs[c], ws);
-            if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(r[i], y);
-            out[size_t(t0 + c) * a.o.ldo] = y;
+      for (int s = 1; s < SPLIT; ++s) v[i] = add4(v[i], part[i][s]);
+    }
+#pragma unroll
+    for (int i = 0; i < TB; ++i) {
+      const int c = cb + 8 * i;
+      if (c >= c_end) break;  // the whole warp
+      const float xs = sxs[c];
+      float y[4] = {i8_value(v[i].x, xs, ws[0]), i8_value(v[i].y, xs, ws[1]), i8_value(v[i].z, xs, ws[2]),
+                    i8_value(v[i].w, xs, ws[3])};
+      if constexpr (EP == B200_EP_SWIGLU) {
+        // Lanes 0..15 hold gate features 4 l .. 4 l + 3, lanes 16..31 the up features of the same
+        // outputs: the lower lane finishes the first two, the upper one the other two.
+        const bool up = lane >= 16;
+        const float a0 = __shfl_xor_sync(0xffffffffu, up ? y[0] : y[2], 16);
+        const float a1 = __shfl_xor_sync(0xffffffffu, up ? y[1] : y[3], 16);
+        if (n0 < a.o.n_valid) {
+          const float g0 = up ? a0 : y[0], g1 = up ? a1 : y[1], u0 = up ? y[2] : a0, u1 = up ? y[3] : a1;
+          const size_t idx = size_t(t0 + c) * a.o.ldo + n0 / 2 + 4 * (lane & 15) + (up ? 2 : 0);
+          if (!LO && a.vec) {
+            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o.out) + idx) = pack_bf16x2(swiglu(g0, u0), swiglu(g1, u1));
+          } else {
+            store_swiglu<LO>(a.o, idx, g0, u0);
+            store_swiglu<LO>(a.o, idx + 1, g1, u1);
           }
+        }
+      } else if (f < a.o.n_valid) {
+        if constexpr (EP == B200_EP_RESID_ADD) {
+          y[0] = __fadd_rn(r[i].x, y[0]);
+          y[1] = __fadd_rn(r[i].y, y[1]);
+          y[2] = __fadd_rn(r[i].z, y[2]);
+          y[3] = __fadd_rn(r[i].w, y[3]);
+        }
+        float* p = static_cast<float*>(a.o.out) + size_t(t0 + c) * a.o.ldo + f;
+        if (a.vec && f + 4 <= a.o.n_valid) {
+          *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (f + e < a.o.n_valid) p[e] = y[e];
         }
       }
     }
   }
-  if (split > 1) cluster_sync_all();  // no CTA leaves while its sums may still be read
+  if (SPLIT > 1) cluster_sync_all();  // no CTA leaves while its sums may still be read
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
@@ -744,28 +787,20 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   return B200_OK;
 }
 
-template <int EP, bool LO>
-static int launch_i8_split(I8Args a, cudaStream_t st) {
+template <int EP, bool LO, int SPLIT>
+static int launch_i8_cluster(const I8Args& a, int n_tiles, int m_tiles, cudaStream_t st) {
   static DeviceOnce attr;
   const int r = once_per_device(attr, [](int) -> int {
-    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<EP, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<EP, LO, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  227 * 1024));
     return B200_OK;
   });
   if (r != B200_OK) return r;
-  const int nk = (a.k + I8_BK - 1) / I8_BK, n_tiles = (a.o.n_valid + 127) / 128;
-  int m_tiles = (a.m + 127) / 128;
-  a.bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
-  m_tiles = (a.m + a.bt - 1) / a.bt;
-  const int tiles = n_tiles * m_tiles;
-  a.split = 1;
-  while (a.split < 8 && 2 * a.split * tiles <= sm_count() && 4 * a.split <= nk) a.split *= 2;
-  const int stage = I8S_OP_W + a.bt * I8_BK;
-  a.stages = std::min({I8S_MAX_STAGES, I8S_SMEM / stage, std::max(4, (nk + a.split - 1) / a.split)});
   CUtensorMap mw, mx;
   if (int rc = i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
   if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, a.bt)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.split * n_tiles, m_tiles);
+  cfg.gridDim = dim3(SPLIT * n_tiles, m_tiles);
   cfg.blockDim = dim3(I8S_THREADS);
   cfg.dynamicSmemBytes = i8s_smem(a.stages, a.bt);
   cfg.stream = st;
@@ -773,12 +808,37 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = a.split;
+  at[1].val.clusterDim.x = SPLIT;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
-  SDB_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<EP, LO>, mw, mx, a));
+  cfg.numAttrs = SPLIT > 1 ? 2 : 1;
+  SDB_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<EP, LO, SPLIT>, mw, mx, a));
   return B200_OK;
+}
+
+template <int EP, bool LO>
+static int launch_i8_split(I8Args a, cudaStream_t st) {
+  const int nk = (a.k + I8_BK - 1) / I8_BK, n_tiles = (a.o.n_valid + 127) / 128;
+  int m_tiles = (a.m + 127) / 128;
+  a.bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
+  m_tiles = (a.m + a.bt - 1) / a.bt;
+  const int tiles = n_tiles * m_tiles;
+  // K split over a cluster while that leaves SMs idle otherwise and every CTA two k-blocks
+  int split = 1;
+  while (split < 8 && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
+  // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 200 x
+  // 12288 x 2048 22.3 -> 15.5 us), or when that ring holds most of the CTA's K anyway (the next
+  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 13.4 -> 7.3 us); else the deeper
+  // ring (96 x 12288 x 2048: 12.2 us against 13.9).
+  const int stage = I8S_OP_W + a.bt * I8_BK, nkb = (nk + split - 1) / split;
+  const bool half = tiles * split > sm_count() || 3 * (I8S_RING_HALF / stage) >= 2 * nkb;
+  a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(2, nkb)});
+  switch (split) {
+    case 1: return launch_i8_cluster<EP, LO, 1>(a, n_tiles, m_tiles, st);
+    case 2: return launch_i8_cluster<EP, LO, 2>(a, n_tiles, m_tiles, st);
+    case 4: return launch_i8_cluster<EP, LO, 4>(a, n_tiles, m_tiles, st);
+    default: return launch_i8_cluster<EP, LO, 8>(a, n_tiles, m_tiles, st);
+  }
 }
 
 template <int EP, int RT, int NT8>
@@ -826,7 +886,8 @@ int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k,
     return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: out is not aligned to its elements");
   if (out->lo_format != B200_LO_BF16 && out->lo_format != B200_LO_E4M3)
     return sdb_fail(B200_ERR_ARG, "b200_linear_int8: unknown lo_format");
-  I8Args a{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx, 1, 0, 0, 1};
+  I8Args a{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx, 1, 0, 0, 0};
+  a.vec = out->ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out->out) & (swiglu ? 7 : 15)) == 0;
   switch (out->epilogue) {
     case B200_EP_STORE: return launch_int8<B200_EP_STORE>(a, st);
     case B200_EP_RESID_ADD: return launch_int8<B200_EP_RESID_ADD>(a, st);

@@ -10,7 +10,7 @@
 //
 // Every row is read once: its elements stay in the registers of the threads that share it while
 // the sum, the maximum and the codes follow one another.
-#include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -43,6 +43,15 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
     for (int i = 0; i < TPR / 32; ++i) v = max(v, part[i]);
   }
   return v;
+}
+
+// |v| as a double, put together from its bits: the conversion instruction runs at a quarter of the
+// rate that these do and took 70 of 185 us at 65536 x 2048. Zeros and subnormals come out as
+// numbers below 2^-126, whose squares (2^-252) are far below the last bit of any eps > 0 they are
+// added to; an infinity or NaN comes out finite, and its row is marked by v itself.
+__device__ __forceinline__ double abs_double(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return __hiloint2double(int((b >> 3) + 0x38000000u), int(b << 29));
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -105,31 +114,40 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_int8_kernel(con
     v[i] = j < n4 ? xr[j] : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   if constexpr (DELTA != ACT_NONE) {
+    // every load before the first store: `sum` may be x or delta
+    float4 d[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = t + TPR * i;
-      if (j < n4) {
-        float4 d;
-        if constexpr (DELTA == B200_ACT_F32) {
-          d = reinterpret_cast<const float4*>(static_cast<const float*>(a.delta) + size_t(row) * a.ldd)[j];
-        } else {
-          const uint2 b = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.delta) + size_t(row) * a.ldd)[j];
-          d = make_float4(bf16x2_lo(b.x), bf16x2_hi(b.x), bf16x2_lo(b.y), bf16x2_hi(b.y));
-        }
-        v[i] = make_float4(v[i].x + d.x, v[i].y + d.y, v[i].z + d.z, v[i].w + d.w);
-        if (a.sum) reinterpret_cast<float4*>(a.sum + size_t(row) * a.lds)[j] = v[i];
+      d[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (DELTA == B200_ACT_F32) {
+        if (j < n4) d[i] = reinterpret_cast<const float4*>(static_cast<const float*>(a.delta) + size_t(row) * a.ldd)[j];
+      } else {
+        uint2 b = make_uint2(0u, 0u);
+        if (j < n4) b = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.delta) + size_t(row) * a.ldd)[j];
+        d[i] = make_float4(bf16x2_lo(b.x), bf16x2_hi(b.x), bf16x2_lo(b.y), bf16x2_hi(b.y));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = make_float4(v[i].x + d[i].x, v[i].y + d[i].y, v[i].z + d[i].z, v[i].w + d[i].w);
+    if (a.sum) {
+      float4* sr = reinterpret_cast<float4*>(a.sum + size_t(row) * a.lds);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = t + TPR * i;
+        if (j < n4) sr[j] = v[i];
       }
     }
   }
-  double ss = 0.0;
+  double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;  // four chains: an fp64 FMA waits on the one before
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    ss += double(v[i].x) * double(v[i].x);
-    ss += double(v[i].y) * double(v[i].y);
-    ss += double(v[i].z) * double(v[i].z);
-    ss += double(v[i].w) * double(v[i].w);
+    s0 = fma(abs_double(v[i].x), abs_double(v[i].x), s0);
+    s1 = fma(abs_double(v[i].y), abs_double(v[i].y), s1);
+    s2 = fma(abs_double(v[i].z), abs_double(v[i].z), s2);
+    s3 = fma(abs_double(v[i].w), abs_double(v[i].w), s3);
   }
-  ss = row_sum<TPR>(ss, psum);
+  const double ss = row_sum<TPR>((s0 + s1) + (s2 + s3), psum);
   const float r = float(rsqrt(ss / double(a.k) + double(a.eps)));
   uint32_t mx = 0u;
 #pragma unroll
@@ -166,32 +184,36 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_int8_kernel(co
   const int row = row_of<TPR>(), t = threadIdx.x % TPR;
   if (row >= a.rows) return;
   const int ng = a.k / E;
+  // all of the row's loads first
+  uint4 raw[NV], low[TYPE == ACT_PLANES ? NV : 1];
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.x) + size_t(row) * a.ldx * (16 / E));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) raw[i] = t + TPR * i < ng ? xr[t + TPR * i] : zero;
+  if constexpr (TYPE == ACT_PLANES) {
+    const uint4* lr = reinterpret_cast<const uint4*>(a.lo + size_t(row) * a.ldx);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) low[i] = t + TPR * i < ng ? lr[t + TPR * i] : zero;
+  }
   float v[NV][E];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int j = t + TPR * i;
+    const uint32_t hw[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    if constexpr (TYPE == B200_ACT_F32) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[i][e] = 0.0f;
-    if (j < ng) {
-      if constexpr (TYPE == B200_ACT_F32) {
-        const float4 f = reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + size_t(row) * a.ldx)[j];
-        v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
-      } else {
-        const uint4 h = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + size_t(row) * a.ldx)[j];
-        const uint32_t hw[4] = {h.x, h.y, h.z, h.w};
+      for (int e = 0; e < 4; ++e) v[i][e] = __uint_as_float(hw[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[i][2 * e] = bf16x2_lo(hw[e]);
+        v[i][2 * e + 1] = bf16x2_hi(hw[e]);
+      }
+      if constexpr (TYPE == ACT_PLANES) {
+        const uint32_t lw[4] = {low[i].x, low[i].y, low[i].z, low[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[i][2 * e] = bf16x2_lo(hw[e]);
-          v[i][2 * e + 1] = bf16x2_hi(hw[e]);
-        }
-        if constexpr (TYPE == ACT_PLANES) {
-          const uint4 l = reinterpret_cast<const uint4*>(a.lo + size_t(row) * a.ldx)[j];
-          const uint32_t lw[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[i][2 * e] += bf16x2_lo(lw[e]);
-            v[i][2 * e + 1] += bf16x2_hi(lw[e]);
-          }
+          v[i][2 * e] += bf16x2_lo(lw[e]);
+          v[i][2 * e + 1] += bf16x2_hi(lw[e]);
         }
       }
     }
@@ -219,30 +241,58 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_int8_kernel(co
   }
 }
 
-// A block per row, of the fewest threads that hold it in 16 float4 each.
-template <int DELTA>
-static int launch_norm(const RowArgs& a, cudaStream_t st) {
-  const dim3 grid(a.rows);
-  if (a.k <= 4 * 128 * 16)
-    SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<128, 16, DELTA>, grid, dim3(128), 0, st, a));
-  else if (a.k <= 4 * 512 * 16)
-    SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<512, 16, DELTA>, grid, dim3(512), 0, st, a));
-  else
-    SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<1024, 16, DELTA>, grid, dim3(1024), 0, st, a));
-  return B200_OK;
+// Threads per row (32: eight rows to a block of 256 threads; else a block per row) and 16-byte
+// groups per thread, for `units` groups a row: the fewest threads that hold the row in 16 groups
+// each (a warp's reductions need no barrier, and its loads are all in flight at once), but four
+// times as many while the device has under 512 threads per SM and the row has work for them.
+struct RowShape {
+  int tpr, nv;
+};
+static RowShape row_shape(int rows, int units) {
+  int tpr = 32;
+  while (tpr < 512 && (units > 16 * tpr || (int64_t(rows) * tpr < 512 * int64_t(sm_count()) && units > tpr))) tpr *= 4;
+  if (units > 16 * tpr) tpr = 1024;
+  int nv = 1;
+  while (nv * tpr < units) nv *= 2;
+  return {tpr, nv};
 }
 
-template <int TYPE>
-static int launch_quant(const RowArgs& a, cudaStream_t st) {
-  constexpr int NV = TYPE == B200_ACT_F32 ? 16 : 8;
-  const dim3 grid(a.rows);
-  if (a.k <= 4 * 128 * 16)
-    SDB_CUDA(launch_pdl(quantize_int8_kernel<128, NV, TYPE>, grid, dim3(128), 0, st, a));
-  else if (a.k <= 4 * 512 * 16)
-    SDB_CUDA(launch_pdl(quantize_int8_kernel<512, NV, TYPE>, grid, dim3(512), 0, st, a));
-  else
-    SDB_CUDA(launch_pdl(quantize_int8_kernel<1024, NV, TYPE>, grid, dim3(1024), 0, st, a));
+template <int DELTA, int TPR, int NV>
+static int launch_norm(const RowArgs& a, cudaStream_t st) {
+  const int rpb = TPR == 32 ? 8 : 1;
+  SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<TPR, NV, DELTA>, dim3((a.rows + rpb - 1) / rpb), dim3(rpb * TPR), 0, st, a));
   return B200_OK;
+}
+template <int TYPE, int TPR, int NV>
+static int launch_quant(const RowArgs& a, cudaStream_t st) {
+  const int rpb = TPR == 32 ? 8 : 1;
+  SDB_CUDA(launch_pdl(quantize_int8_kernel<TPR, NV, TYPE>, dim3((a.rows + rpb - 1) / rpb), dim3(rpb * TPR), 0, st, a));
+  return B200_OK;
+}
+template <bool NORM, int KIND, int TPR>
+static int launch_nv(const RowArgs& a, int nv, cudaStream_t st) {
+  auto go = [&](auto n) {
+    if constexpr (NORM) return launch_norm<KIND, TPR, decltype(n)::value>(a, st);
+    else return launch_quant<KIND, TPR, decltype(n)::value>(a, st);
+  };
+  if constexpr (TPR == 1024) return go(std::integral_constant<int, 16>{});  // only rows no block of 512 holds
+  switch (nv) {
+    case 1: return go(std::integral_constant<int, 1>{});
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 4: return go(std::integral_constant<int, 4>{});
+    case 8: return go(std::integral_constant<int, 8>{});
+    default: return go(std::integral_constant<int, 16>{});
+  }
+}
+template <bool NORM, int KIND>
+static int launch_rows(const RowArgs& a, cudaStream_t st) {
+  const RowShape r = row_shape(a.rows, a.k / (NORM || KIND == B200_ACT_F32 ? 4 : 8));
+  switch (r.tpr) {
+    case 32: return launch_nv<NORM, KIND, 32>(a, r.nv, st);
+    case 128: return launch_nv<NORM, KIND, 128>(a, r.nv, st);
+    case 512: return launch_nv<NORM, KIND, 512>(a, r.nv, st);
+    default: return launch_nv<NORM, KIND, 1024>(a, r.nv, st);
+  }
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -270,8 +320,8 @@ int sdb_quantize_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t
   a.ldq = ldq;
   a.rows = rows;
   a.k = k;
-  if (type == B200_ACT_F32) return launch_quant<B200_ACT_F32>(a, st);
-  return x_lo ? launch_quant<ACT_PLANES>(a, st) : launch_quant<B200_ACT_BF16>(a, st);
+  if (type == B200_ACT_F32) return launch_rows<false, B200_ACT_F32>(a, st);
+  return x_lo ? launch_rows<false, ACT_PLANES>(a, st) : launch_rows<false, B200_ACT_BF16>(a, st);
 }
 
 int sdb_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd, float* sum,
@@ -281,7 +331,7 @@ int sdb_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t del
   if (sum && !delta) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: sum needs a delta");
   if (delta && delta_type != B200_ACT_F32 && delta_type != B200_ACT_BF16)
     return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: unknown delta type");
-  if (!(eps >= 0.0f)) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: eps must not be negative");
+  if (!(eps > 0.0f)) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: eps must be positive");
   if (rows <= 0 || hidden <= 0) return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: empty shape");
   if (hidden % 16 != 0 || hidden > I8_K_MAX)
     return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: hidden must be a multiple of 16, at most 65536");
@@ -306,8 +356,8 @@ int sdb_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t del
   a.rows = rows;
   a.k = hidden;
   a.eps = eps;
-  if (!delta) return launch_norm<ACT_NONE>(a, st);
-  return delta_type == B200_ACT_F32 ? launch_norm<B200_ACT_F32>(a, st) : launch_norm<B200_ACT_BF16>(a, st);
+  if (!delta) return launch_rows<true, ACT_NONE>(a, st);
+  return delta_type == B200_ACT_F32 ? launch_rows<true, B200_ACT_F32>(a, st) : launch_rows<true, B200_ACT_BF16>(a, st);
 }
 
 }  // namespace sdb

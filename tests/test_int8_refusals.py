@@ -72,6 +72,7 @@ def test_rmsnorm_int8(lib, p16):
     bad(1, delta=None)                   # a sum of nothing
     bad(1, dt=3)
     bad(1, eps=-1e-6)
+    bad(1, eps=0.0)
     bad(1, eps=float("nan"))
     bad(2, rows=0)
     bad(2, k=0)
