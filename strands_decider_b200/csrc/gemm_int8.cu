@@ -614,10 +614,7 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
 // g + 8 (a quad reads 64 neighbouring bytes), and of tokens g and g + 8. mma.sync m16n8k32 takes 4
 // codes of each row per register: MMA j = 0, 1 is given the words 2 j and 2 j + 1 of both operands,
 // so its k-slots are the same columns on both sides, in an order the sum does not see.
-constexpr int I8R_THREADS = 256;
-constexpr int I8R_WARPS = I8R_THREADS / 32;
 constexpr int I8R_MAX_M = 16;
-constexpr int I8R_DEPTH = 4;  // k-blocks in flight per warp
 
 __device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
@@ -635,10 +632,10 @@ __device__ __forceinline__ uint4 ld_stream_u4(const void* p) {
   return v;
 }
 
-template <int EP, int RT, int NT8>
-__global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Args a) {
+template <int EP, int RT, int NT8, int W, int D, int CTAS>
+__global__ void __launch_bounds__(32 * W, CTAS) gemm_i8_reg_kernel(const I8Args a) {
   static_assert(EP != B200_EP_SWIGLU || RT == 2, "a SwiGLU CTA holds a gate tile and its up tile");
-  __shared__ int4 red[I8R_WARPS][RT][NT8][32];
+  __shared__ int4 red[W][RT][NT8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int nkb = (a.k + 63) / 64;
   int row0[RT];
@@ -656,12 +653,12 @@ __global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Arg
   pdl_wait();
   pdl_trigger();
 
-  const int ns = warp < nkb ? (nkb - warp + I8R_WARPS - 1) / I8R_WARPS : 0;
-  uint4 wr[I8R_DEPTH][RT][2], xr[I8R_DEPTH][NT8];
+  const int ns = warp < nkb ? (nkb - warp + W - 1) / W : 0;
+  uint4 wr[D][RT][2], xr[D][NT8];
   int acc[RT][NT8][4] = {};
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   auto load = [&](int d, int s) {
-    const int k0 = (warp + I8R_WARPS * s) * 64 + 16 * t;
+    const int k0 = (warp + W * s) * 64 + 16 * t;
     const bool in = k0 < a.k;  // k is a multiple of 16: a lane's 16 codes are all inside or all outside
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -677,11 +674,33 @@ __global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Arg
     }
   };
 #pragma unroll
-  for (int d = 0; d < I8R_DEPTH; ++d)
+  for (int d = 0; d < D; ++d)
     if (d < ns) load(d, d);
-  for (int s0 = 0; s0 < ns; s0 += I8R_DEPTH) {
+  // what a finishing warp needs besides the sums: lane (g, t) finishes row g (e = 0, 1) and g + 8
+  // (e = 2, 3) of tile rt for tokens 2 t (e = 0, 2) and 2 t + 1 of token tile i
+  constexpr int SETS = (EP == B200_EP_SWIGLU ? 1 : RT) * NT8;  // (tile, 8 tokens) finished by a warp each
+  const int rt = warp < SETS ? warp / NT8 : 0, i = warp % NT8;
+  const int first = rt ? row0[RT - 1] : row0[0];
+  float xs[2] = {}, ws[2] = {}, wu[2] = {}, res[4] = {};
+  if (warp < SETS) {
 #pragma unroll
-    for (int d = 0; d < I8R_DEPTH; ++d) {
+    for (int e = 0; e < 2; ++e) {
+      const int tok = 8 * i + 2 * t + e, n = first + g + 8 * e;
+      xs[e] = tok < a.m ? a.xs[tok] : 0.0f;
+      ws[e] = n < a.n ? a.ws[n] : 0.0f;
+      if constexpr (EP == B200_EP_SWIGLU) wu[e] = a.ws[row0[RT - 1] + g + 8 * e];
+    }
+    if constexpr (EP == B200_EP_RESID_ADD) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = 8 * i + 2 * t + (e & 1), n = first + g + 8 * (e >> 1);
+        if (tok < a.m && n < a.o.n_valid) res[e] = static_cast<const float*>(a.o.out)[size_t(tok) * a.o.ldo + n];
+      }
+    }
+  }
+  for (int s0 = 0; s0 < ns; s0 += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
       if (s0 + d < ns) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -691,7 +710,7 @@ __global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Arg
             mma_s8_16832(acc[rt][i], u.x, v.x, u.y, v.y, x.x, x.y);
             mma_s8_16832(acc[rt][i], u.z, v.z, u.w, v.w, x.z, x.w);
           }
-        if (s0 + d + I8R_DEPTH < ns) load(d, s0 + d + I8R_DEPTH);
+        if (s0 + d + D < ns) load(d, s0 + d + D);
       }
     }
   }
@@ -701,18 +720,15 @@ __global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Arg
     for (int i = 0; i < NT8; ++i)
       red[warp][rt][i][lane] = make_int4(acc[rt][i][0], acc[rt][i][1], acc[rt][i][2], acc[rt][i][3]);
   __syncthreads();
-  constexpr int SETS = (EP == B200_EP_SWIGLU ? 1 : RT) * NT8;  // (tile, 8 tokens) finished by a warp each
   if (warp >= SETS) return;
-  const int rt = warp / NT8, i = warp % NT8;
   auto sums = [&](int r, int (&v)[4]) {
     v[0] = v[1] = v[2] = v[3] = 0;
 #pragma unroll
-    for (int w = 0; w < I8R_WARPS; ++w) {
+    for (int w = 0; w < W; ++w) {
       const int4 p = red[w][r][i][lane];
       v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
     }
   };
-  // lane (g, t) holds row g, tokens 2t and 2t + 1, then row g + 8
   int v[4];
   sums(rt, v);
   if constexpr (EP == B200_EP_SWIGLU) {
@@ -722,21 +738,19 @@ __global__ void __launch_bounds__(I8R_THREADS, 2) gemm_i8_reg_kernel(const I8Arg
     for (int e = 0; e < 4; ++e) {
       const int tok = 8 * i + 2 * t + (e & 1), l = g + 8 * (e >> 1);
       if (tok >= a.m) continue;
-      const float xs = a.xs[tok];
-      const float g = i8_value(v[e], xs, a.ws[row0[0] + l]), up = i8_value(u[e], xs, a.ws[row0[1] + l]);
+      const float gv = i8_value(v[e], xs[e & 1], ws[e >> 1]), uv = i8_value(u[e], xs[e & 1], wu[e >> 1]);
       const size_t idx = size_t(tok) * a.o.ldo + (blockIdx.x >> 2) * 64 + (blockIdx.x & 3) * 16 + l;
-      if (a.o.lo_offset) store_swiglu<true>(a.o, idx, g, up);
-      else store_swiglu<false>(a.o, idx, g, up);
+      if (a.o.lo_offset) store_swiglu<true>(a.o, idx, gv, uv);
+      else store_swiglu<false>(a.o, idx, gv, uv);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int tok = 8 * i + 2 * t + (e & 1), n = row0[rt] + g + 8 * (e >> 1);
+      const int tok = 8 * i + 2 * t + (e & 1), n = first + g + 8 * (e >> 1);
       if (tok >= a.m || n >= a.o.n_valid) continue;
-      float* p = static_cast<float*>(a.o.out) + size_t(tok) * a.o.ldo + n;
-      float y = i8_value(v[e], a.xs[tok], a.ws[n]);
-      if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(*p, y);
-      *p = y;
+      float y = i8_value(v[e], xs[e & 1], ws[e >> 1]);
+      if constexpr (EP == B200_EP_RESID_ADD) y = __fadd_rn(res[e], y);
+      static_cast<float*>(a.o.out)[size_t(tok) * a.o.ldo + n] = y;
     }
   }
 }
@@ -841,18 +855,35 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   }
 }
 
-template <int EP, int RT, int NT8>
+template <int EP, int RT, int NT8, int W, int D, int CTAS>
 static int launch_i8_reg(const I8Args& a, cudaStream_t st) {
   const int grid = (a.o.n_valid + 16 * RT - 1) / (16 * RT);
-  SDB_CUDA(launch_pdl(gemm_i8_reg_kernel<EP, RT, NT8>, dim3(grid), dim3(I8R_THREADS), 0, st, a));
+  SDB_CUDA(launch_pdl(gemm_i8_reg_kernel<EP, RT, NT8, W, D, CTAS>, dim3(grid), dim3(32 * W), 0, st, a));
   return B200_OK;
+}
+// Warps per CTA, depth and CTAs per SM, each the best of the shapes measured beside it (us):
+//   SwiGLU, 12288 x 2048: 1 token 6.4 (others 7.7 - 9.9), 16 tokens 8.8 (10.2 - 11.0)
+//   few tiles (about one CTA per SM), deep K: 16 warps share it (2048 x 6144, 1 token 4.0 against
+//   6.9 on 8 warps); shallow K: 8 warps (2048 x 2048, 13 tokens 3.2 against 3.9 on 16)
+//   many tiles, 8224 x 2048: 1 token 4.8 (6.2 - 8.6), 16 tokens two tiles per CTA 5.8 (6.9 - 9.6)
+template <int EP, int NT8>
+static int dispatch_i8_reg(const I8Args& a, cudaStream_t st) {
+  if constexpr (EP == B200_EP_SWIGLU) {
+    if constexpr (NT8 == 1) return launch_i8_reg<EP, 2, NT8, 8, 2, 3>(a, st);
+    else return launch_i8_reg<EP, 2, NT8, 4, 4, 4>(a, st);
+  } else {
+    if ((a.o.n_valid + 15) / 16 <= 2 * sm_count())
+      return a.k >= 4096 ? launch_i8_reg<EP, 1, NT8, 16, NT8 == 1 ? 6 : 4, 1>(a, st)
+                         : launch_i8_reg<EP, 1, NT8, 8, 4, 2>(a, st);
+    if constexpr (NT8 == 1) return launch_i8_reg<EP, 1, NT8, 8, 3, 3>(a, st);
+    else return launch_i8_reg<EP, 2, NT8, 8, 2, 2>(a, st);
+  }
 }
 
 template <int EP>
 static int launch_int8(const I8Args& a, cudaStream_t st) {
-  constexpr int RT = EP == B200_EP_SWIGLU ? 2 : 1;
-  if (a.m <= 8) return launch_i8_reg<EP, RT, 1>(a, st);
-  if (a.m <= I8R_MAX_M) return launch_i8_reg<EP, RT, 2>(a, st);
+  if (a.m <= 8) return dispatch_i8_reg<EP, 1>(a, st);
+  if (a.m <= I8R_MAX_M) return dispatch_i8_reg<EP, 2>(a, st);
   // pairs once every pair has a whole tile
   const int64_t units = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
   const bool pairs = units >= sm_count() / 2;
