@@ -115,6 +115,20 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, i
                : "memory");
 }
 
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_addr(src)), "r"(x), "r"(y)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// All but the newest N of this thread's stores have read their shared memory.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tma_store_wait_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ----------------------------------------------------------------------------- CTA pairs
 // Tile: 256 features (128 per CTA) x 256 tokens, K in stages of 128 codes (four MMAs of K = 32).
 // Each CTA loads its 128 weight rows and its half of the tokens; the pair's MMA reads both halves.
@@ -127,17 +141,23 @@ constexpr int I8P_EPI_WARPS = 8;
 constexpr int I8P_XCH_LD = 20;  // floats per lane of an exchange buffer (16 tokens; 16-byte accesses
                                 // of 8 neighbouring lanes then fall into different banks)
 
-template <int EP>
+// How the pair kernel writes: from registers (any alignment), the SwiGLU with a low plane, or 16
+// tokens x 32 features at a time from shared memory by TMA (16-byte aligned rows: stores of 4
+// bytes, or 2 of the SwiGLU, and their addresses were the longest part of the epilogue).
+enum I8Out { I8_DIRECT = 0, I8_PLANES = 1, I8_TMA = 2 };
+
+template <int EP, int OUT>
 struct I8PairSmem {
   static constexpr int OP = 128 * I8_BK;                    // one operand of a stage
   static constexpr int STAGE = 2 * OP;
-  // the SwiGLU gives one stage for the exchange of gate and up sums between lane halves:
-  // [round parity][token half, feature half][side][lane][16 tokens]
-  static constexpr int STAGES = EP == B200_EP_SWIGLU ? 5 : 6;
+  // one stage goes to the tiles of TMA stores, or to the SwiGLU's exchange of gate and up sums
+  // between lane halves: [round parity][token half, feature half][side][lane][16 tokens]
+  static constexpr int STAGES = EP == B200_EP_SWIGLU || OUT == I8_TMA ? 5 : 6;
+  static constexpr int OT = OUT == I8_TMA ? 16 * 32 * (EP == B200_EP_SWIGLU ? 2 : 4) : 0;  // one tile of a store
   static constexpr int XCH = EP == B200_EP_SWIGLU ? 2 * 4 * 2 * 32 * I8P_XCH_LD * 4 : 0;
   static constexpr int XS = I8P_EPI_WARPS * 128 * 4;        // each epilogue warp's token scales
   static constexpr int BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = 1024 + STAGES * STAGE + XCH + XS + BARS * 8 + 16;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE + 2 * I8P_EPI_WARPS * OT + XCH + XS + BARS * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -159,16 +179,17 @@ __device__ __forceinline__ void i8_finish(const I8Args& a, const uint32_t (&v)[C
   }
 }
 
-template <int EP, bool LO>
+template <int EP, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                        const I8Args a) {
-  using SM = I8PairSmem<EP>;
+                        const __grid_constant__ CUtensorMap tmO, const I8Args a) {
+  using SM = I8PairSmem<EP, OUT>;
   extern __shared__ uint8_t i8_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = sW + SM::STAGES * SM::OP;
-  float* xch = reinterpret_cast<float*>(sX + SM::STAGES * SM::OP);
+  uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp][2] tiles of TMA stores
+  float* xch = reinterpret_cast<float*>(sO + 2 * I8P_EPI_WARPS * SM::OT);
   float* sxs = xch + SM::XCH / 4;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxs + SM::XS / 4);
   uint64_t* full = bars;                            // the leader's are used
@@ -269,6 +290,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     const int q = warp & 3, hf = (warp - 2) >> 2;
     const uint32_t acc_empty0 = mapa_shared(smem_addr(acc_empty), 0);
     float* xs = sxs + (warp - 2) * 128;  // scales of this warp's 128 tokens
+    uint8_t* tiles = sO + 2 * (warp - 2) * SM::OT;
+    auto tile_free = [&]() {  // the tile about to be filled was read by its last store
+      if constexpr (OUT == I8_TMA) {
+        if (lane == 0) tma_store_wait_read<1>();
+        __syncwarp();
+      }
+    };
+    auto tile_store = [&](int which, int x, int y) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tma_store_2d(&tmO, tiles + which * SM::OT, x, y);
+    };
     uint32_t local = 0;
     for (int u = pair; u < n_units; u += n_pairs, ++local) {
       int mt, nt;
@@ -317,10 +350,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
                 make_float4(i8_value(int(vs[c & 1][j]), x.x, ws), i8_value(int(vs[c & 1][j + 1]), x.y, ws),
                             i8_value(int(vs[c & 1][j + 2]), x.z, ws), i8_value(int(vs[c & 1][j + 3]), x.w, ws));
           }
+          tile_free();
           asm volatile("bar.sync %0, 64;" ::"r"(1 + grp) : "memory");
           if (valid) {
             const int l = left - 32 * c - oc;  // of these 16 tokens, the ones inside the batch
             const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
+            uint16_t* tile = reinterpret_cast<uint16_t*>(tiles + (c & 1) * SM::OT) + lane;
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
               const float4 x = *reinterpret_cast<const float4*>(xc + oc + j);
@@ -329,16 +364,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float own = i8_value(int(vo[c & 1][j + e]), xe[e], ws);
-                if (j + e < l)
-                  store_swiglu<LO>(a.o, idx + size_t(j + e) * a.o.ldo, side ? oe[e] : own, side ? own : oe[e]);
+                const float gv = side ? oe[e] : own, uv = side ? own : oe[e];
+                if constexpr (OUT == I8_TMA) tile[32 * (j + e)] = f32_to_bf16_rn(swiglu(gv, uv));
+                else if (j + e < l) store_swiglu<OUT == I8_PLANES>(a.o, idx + size_t(j + e) * a.o.ldo, gv, uv);
               }
+            }
+            if constexpr (OUT == I8_TMA) {
+              if (l > 0) tile_store(c & 1, n0 / 2 + 32 * (q & 1), t0 + 32 * c + oc);
             }
           }
         }
       } else {
         float* p = static_cast<float*>(a.o.out) + size_t(t0) * a.o.ldo + n;
         const bool valid = n < a.o.n_valid;
-        constexpr int CW = EP == B200_EP_RESID_ADD ? 16 : 32;  // columns in hand (and as many ahead)
+        // columns in hand (and as many ahead)
+        constexpr int CW = EP == B200_EP_RESID_ADD || OUT == I8_TMA ? 16 : 32;
         float r[2][CW];
         auto residual = [&](int c) {  // chunk c's residual, read while the chunk before is finished
           if constexpr (EP == B200_EP_RESID_ADD) {
@@ -359,9 +399,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
             tmem_ld(tl + CW * (c + 1), v[(c + 1) & 1]);
             residual(c + 1);
           }
-          if (valid) {
+          const int l = left - CW * c;
+          if constexpr (OUT == I8_TMA) {
+            tile_free();
+            float* tile = reinterpret_cast<float*>(tiles + (c & 1) * SM::OT) + lane;
+#pragma unroll
+            for (int j = 0; j < CW; j += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(xs + CW * c + j);
+              tile[32 * j] = i8_value(int(v[c & 1][j]), x.x, ws);
+              tile[32 * (j + 1)] = i8_value(int(v[c & 1][j + 1]), x.y, ws);
+              tile[32 * (j + 2)] = i8_value(int(v[c & 1][j + 2]), x.z, ws);
+              tile[32 * (j + 3)] = i8_value(int(v[c & 1][j + 3]), x.w, ws);
+            }
+            if (l > 0 && n0 + 32 * q < a.o.n_valid) tile_store(c & 1, n0 + 32 * q, t0 + CW * c);
+          } else if (valid) {
             float* pc = p + size_t(CW * c) * a.o.ldo;
-            const int l = left - CW * c;
             if (l >= CW) i8_finish<EP, true>(a, v[c & 1], xs + CW * c, ws, pc, r[c & 1], l);
             else i8_finish<EP, false>(a, v[c & 1], xs + CW * c, ws, pc, r[c & 1], l);
           }
@@ -374,6 +426,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     }
   }
 
+  if constexpr (OUT == I8_TMA) {
+    if (warp >= 2 && lane == 0) tma_store_wait_done();
+  }
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves while the other may still read or signal it
   if (warp == 1) {
@@ -765,19 +820,19 @@ static int i8_map(CUtensorMap* map, const void* base, int rows, int k, int ld, i
   return encode_bf16_sw128(map, base, 2, dims, strides, box);
 }
 
-template <int EP, bool LO>
+template <int EP, int OUT>
 static int launch_i8_pair(I8Args a, cudaStream_t st) {
-  constexpr int smem = I8PairSmem<EP>::TOTAL;
+  constexpr int smem = I8PairSmem<EP, OUT>::TOTAL;
   static DeviceOnce attr;
   static int max_pairs_dev[kMaxDevices] = {};  // written under attr's lock, once per device
   const int r = once_per_device(attr, [](int dev) -> int {
-    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<EP, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SDB_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<EP, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sm_count() & ~1);
     cfg.blockDim = dim3(I8P_THREADS);
     cfg.dynamicSmemBytes = smem;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<EP, LO>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<EP, OUT>, &cfg) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = sm_count() / 2;
     }
@@ -787,17 +842,23 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   if (r != B200_OK) return r;
   int dev = 0;
   SDB_CUDA(cudaGetDevice(&dev));
-  CUtensorMap mw, mx;
+  CUtensorMap mw, mx, mo;
   if (int rc = i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
   if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, 128)) return rc;
+  constexpr bool SW = EP == B200_EP_SWIGLU;
+  mo = mw;  // not read
+  if constexpr (OUT == I8_TMA) {
+    if (int rc = encode_store_tile(&mo, a.o.out, SW ? 2 : 4, a.m, SW ? a.o.n_valid / 2 : a.o.n_valid, a.o.ldo, 16, 32))
+      return rc;
+  }
   const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + 255) / 256;
   // weights beyond what L2 keeps beside the activation stream: groups of about 40 MB
   const double tile_bytes = 256.0 * a.k;
   const int groups = n_tiles * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles * tile_bytes / 40e6));
   a.ngroup = (n_tiles + groups - 1) / groups;
   const int units = n_tiles * m_tiles;
-  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP, LO>, dim3(2 * std::min(units, max_pairs_dev[dev])), dim3(I8P_THREADS), smem,
-                      st, mw, mx, a));
+  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP, OUT>, dim3(2 * std::min(units, max_pairs_dev[dev])), dim3(I8P_THREADS), smem,
+                      st, mw, mx, mo, a));
   return B200_OK;
 }
 
@@ -870,12 +931,12 @@ template <int EP, int NT8>
 static int dispatch_i8_reg(const I8Args& a, cudaStream_t st) {
   if constexpr (EP == B200_EP_SWIGLU) {
     if constexpr (NT8 == 1) return launch_i8_reg<EP, 2, NT8, 8, 2, 3>(a, st);
-    else return launch_i8_reg<EP, 2, NT8, 4, 4, 4>(a, st);
+    else return launch_i8_reg<EP, 2, NT8, 4, 3, 4>(a, st);
   } else {
     if ((a.o.n_valid + 15) / 16 <= 2 * sm_count())
       return a.k >= 4096 ? launch_i8_reg<EP, 1, NT8, 16, NT8 == 1 ? 6 : 4, 1>(a, st)
                          : launch_i8_reg<EP, 1, NT8, 8, 4, 2>(a, st);
-    if constexpr (NT8 == 1) return launch_i8_reg<EP, 1, NT8, 8, 3, 3>(a, st);
+    if constexpr (NT8 == 1) return launch_i8_reg<EP, 1, NT8, 8, 2, 4>(a, st);
     else return launch_i8_reg<EP, 2, NT8, 8, 2, 2>(a, st);
   }
 }
@@ -886,11 +947,21 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   if (a.m <= I8R_MAX_M) return dispatch_i8_reg<EP, 2>(a, st);
   // pairs once every pair has a whole tile
   const int64_t units = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
-  const bool pairs = units >= sm_count() / 2;
-  if constexpr (EP == B200_EP_SWIGLU) {
-    if (a.o.lo_offset) return pairs ? launch_i8_pair<EP, true>(a, st) : launch_i8_split<EP, true>(a, st);
+  constexpr bool SW = EP == B200_EP_SWIGLU;
+  if (units < sm_count() / 2) {
+    if constexpr (SW) {
+      if (a.o.lo_offset) return launch_i8_split<EP, true>(a, st);
+    }
+    return launch_i8_split<EP, false>(a, st);
   }
-  return pairs ? launch_i8_pair<EP, false>(a, st) : launch_i8_split<EP, false>(a, st);
+  if constexpr (SW) {
+    if (a.o.lo_offset) return launch_i8_pair<EP, I8_PLANES>(a, st);
+  }
+  if constexpr (EP != B200_EP_RESID_ADD) {
+    if (int64_t(a.o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o.out) & 15) == 0)
+      return launch_i8_pair<EP, I8_TMA>(a, st);
+  }
+  return launch_i8_pair<EP, I8_DIRECT>(a, st);
 }
 
 int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
