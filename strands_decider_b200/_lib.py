@@ -182,7 +182,7 @@ def check(status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    check(getattr(_lib or load(), name)(*args))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -196,6 +196,12 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def raw_stream(device: int) -> int:
+    """The cudaStream_t of a device's current stream, without a torch.cuda.Stream made for it (2 us
+    of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def split_planes(x: torch.Tensor) -> torch.Tensor:
