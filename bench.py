@@ -210,7 +210,11 @@ def launches_per_forward(spec: config.ModelSpec, decide: bool, tokens: int = 0, 
     mixer's 2 kernels, plus a zeroing kernel before a split-K in-projection (batches of 129 to
     4095 tokens; up to 128 tokens on packed weights the norm before it clears the output);
     forwards of >= 4096 tokens also dequantise each of the 4 weights per layer once (bf16
-    weights too with the e4m3 low plane); the slot-length update when states are saved; the head."""
+    weights too with the e4m3 low plane); the slot-length update when states are saved; the head.
+    Int8 weights (W8A8): per layer 2 norms, 4 GEMMs, the mixer's 2 kernels and 2 activation
+    quantisers at every size."""
+    if spec.weight_format == "int8":
+        return 1 + (1 if decide else 0) + (1 if saves else 0) + 10 * len(spec.layer_types)
     big = tokens >= 4096
     folded = tokens <= 128 and spec.weight_format != "bf16"
     dq = 4 if big and (spec.weight_format != "bf16" or lo_plane == "e4m3") else 0
@@ -434,7 +438,8 @@ def _case_profiled(fn) -> None:
 def gemm_case(m: int, fmt: str, ep: str, n: int = 2 * 6144, k: int = 2048, planes: str = "split"):
     """b200_linear with x as two bf16 planes [2, m, k] and a packed [n, k] weight; with planes
     "lo8", b200_linear_lo8 on the weight's two copies (b200_dequantize_lo8) and an e4m3 low
-    plane, as large batches run it with lo_plane "e4m3"."""
+    plane, as large batches run it with lo_plane "e4m3"; with fmt "int8", b200_linear_int8 on
+    int8 codes (`planes` is not used)."""
     g = torch.Generator(device="cuda").manual_seed(0)
     if ep == "swiglu":
         gate = WT.quantize(fmt, torch.randn(n // 2, k, device="cuda", generator=g) * 0.02)
@@ -452,6 +457,13 @@ def gemm_case(m: int, fmt: str, ep: str, n: int = 2 * 6144, k: int = 2048, plane
         o = _lib.LinearOut(_lib.EP_STORE if ep == "store" else _lib.EP_RESID_ADD, n, _lib.ptr(out), n, 0)
     qw = pw.qweight()
     keep = (pw, xp, out)
+    if fmt == "int8":
+        from strands_decider_b200 import int8
+
+        codes, scale = int8.quantize_act(xp[0], lo=xp[1])
+        dst = out[0] if ep == "swiglu" else out
+        name = {"swiglu": "swiglu", "store": "store", "resid": "residual"}[ep]
+        return lambda: int8.linear(codes, scale, pw, dst, epilogue=name, n_valid=n), 2.0 * m * n * k
     if planes == "lo8":
         whi = torch.empty(pw.n, k, dtype=torch.bfloat16, device="cuda")
         wlo8 = torch.empty(pw.n, k, dtype=torch.uint8, device="cuda")

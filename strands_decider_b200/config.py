@@ -22,7 +22,7 @@ from dataclasses import dataclass, field, replace
 GDN = "linear_attention"
 ATTN = "full_attention"
 
-WEIGHT_FORMATS = ("bf16", "int4", "nvfp4", "ternary")
+WEIGHT_FORMATS = ("bf16", "int4", "nvfp4", "ternary", "int8")   # int8: activations in int8 too (W8A8)
 ROW_PAD = 256          # fused weights are padded to this many rows (the GEMM's widest N tile)
 SWIGLU_BLOCK = 64      # gate/up interleave block
 

@@ -58,6 +58,13 @@ int sdb_rmsnorm(const float* x, int32_t rows, int32_t hidden, const float* w, fl
 bool rmsnorm_folds_zero(int32_t rows, int32_t hidden);
 namespace sdb {
 bool linear_small_m(int32_t m, int32_t format);
+int sdb_quantize_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t rows, int32_t k, int32_t ldx,
+                      int8_t* q, int32_t ldq, float* scale, cudaStream_t st);
+int sdb_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd, float* sum,
+                     int32_t lds, int32_t rows, int32_t hidden, const float* w, float eps, int8_t* q, int32_t ldq,
+                     float* scale, cudaStream_t st);
+int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
+                    const b200_linear_out* out, cudaStream_t st);
 }  // namespace sdb
 
 extern "C" const char* b200_last_error(void) { return g_last_error.c_str(); }
@@ -98,7 +105,10 @@ struct b200_model {
       if (cfg.layer_kind[i] == B200_LAYER_GDN) return true;
     return false;
   }
+  // W8A8: int8 activation codes and int8 weights, nothing to unpack
+  bool int8() const { return cfg.weight_format == B200_W_INT8; }
   bool dequant_at(int T) const {
+    if (int8()) return false;
     const int from = cfg.dequant_min_tokens == 0 ? 4096 : cfg.dequant_min_tokens;
     return from > 0 && T >= from;
   }
@@ -122,9 +132,11 @@ namespace {
 //   prep fp32                        GDN scratch (conv / l2norm / gating outputs)
 //   wdq  bf16 [N, K]                 one dequantised weight (batches of >= dequant_min_tokens)
 //   wdq8 e4m3 [N, K]                 its e4m3 copy (lo_format B200_LO_E4M3)
+//   int8 weights: xn holds int8 codes [T, hidden] instead; xs, as fp32 [T] are the token scales
+//   of xn and of aq int8 [T, act_cols], the codes of act
 // With e4m3 low planes the xn / act lo planes hold one byte per element in the same space.
 struct WsLayout {
-  size_t x, xn, mix, act, q, k, v, prep, wdq, wdq8, total;
+  size_t x, xn, mix, act, q, k, v, prep, wdq, wdq8, xs, aq, as, total;
   int mix_cols, act_cols;
   long long xn_lo, act_lo;  // element offsets of the lo planes
 };
@@ -146,7 +158,7 @@ WsLayout layout(const b200_model& m, int T) {
   };
   L.x = take(size_t(T) * c.hidden * 4);
   const size_t xn_plane = align256(size_t(T) * c.hidden * 2);
-  L.xn = take(2 * xn_plane);
+  L.xn = take(m.int8() ? size_t(T) * c.hidden : 2 * xn_plane);
   L.xn_lo = (long long)(xn_plane / 2);
   L.mix = take(size_t(T) * L.mix_cols * 4);
   const size_t act_plane = align256(size_t(T) * L.act_cols * 2);
@@ -157,6 +169,11 @@ WsLayout layout(const b200_model& m, int T) {
   L.k = take(kvb);
   L.v = take(kvb);
   L.prep = take(m.has_gdn() ? size_t(sdb_gdn_prep_floats(c.gdn_heads, T)) * 4 : 16);
+  if (m.int8()) {
+    L.xs = take(size_t(T) * 4);
+    L.aq = take(size_t(T) * L.act_cols);
+    L.as = take(size_t(T) * 4);
+  }
   L.wdq = 0;
   if (m.dequant_at(T)) {
     size_t most = 0;
@@ -193,10 +210,64 @@ int run_linear(const b200_model& m, const uint16_t* x, const uint16_t* x_lo, int
   return b200_linear(x, x_lo, T, k, k, &w, &o, stream);
 }
 
-int check_qw(const b200_qweight& w, int n_min, int k, const char* what) {
+// A layer of an int8 model: the norms and the outputs of the mixer and the SwiGLU as int8 codes
+// with a scale per token, every linear on them (TF:747-783 otherwise as below).
+int forward_layer_int8(const b200_model& m, int li, const b200_seqs* seqs, const b200_prefix_pool* pool, const WsLayout& L,
+                       uint8_t* ws, cudaStream_t st) {
+  const auto& c = m.cfg;
+  const b200_layer_weights& w = m.layers[li];
+  const int T = seqs->n_tokens;
+  float* x = reinterpret_cast<float*>(ws + L.x);
+  float* mix = reinterpret_cast<float*>(ws + L.mix);
+  uint16_t* act = reinterpret_cast<uint16_t*>(ws + L.act);
+  int8_t* xq = reinterpret_cast<int8_t*>(ws + L.xn);
+  float* xs = reinterpret_cast<float*>(ws + L.xs);
+  int8_t* aq = reinterpret_cast<int8_t*>(ws + L.aq);
+  float* as = reinterpret_cast<float*>(ws + L.as);
+  auto norm = [&](const float* nw) {
+    return sdb::sdb_rmsnorm_int8(x, c.hidden, nullptr, 0, 0, nullptr, 0, T, c.hidden, nw, c.eps, xq, c.hidden, xs, st);
+  };
+  auto linear = [&](const int8_t* q, const float* s, int k, const b200_qweight& qw, int ep, int n, void* out, int ldo) {
+    const b200_linear_out o{ep, n, out, ldo, 0, 0};
+    return sdb::sdb_linear_int8(q, s, T, k, k, &qw, &o, st);
+  };
+  int rc;
+  if ((rc = norm(w.input_norm))) return rc;
+  int k_out;
+  if (c.layer_kind[li] == B200_LAYER_GDN) {
+    const int n = m.gdn_in_cols();
+    if ((rc = linear(xq, xs, c.hidden, w.mix_in, B200_EP_STORE, n, mix, n))) return rc;
+    if ((rc = sdb_gdn_mixer(&w.gdn, seqs, mix, n, act, L.act_lo, pool, m.kind_index[li],
+                            reinterpret_cast<float*>(ws + L.prep), 0, st)))
+      return rc;
+    k_out = m.value_dim();
+  } else {
+    const int n = m.attn_qkv();
+    if ((rc = linear(xq, xs, c.hidden, w.mix_in, B200_EP_STORE, n, mix, n))) return rc;
+    const b200_attn_params ap{c.attn_heads, c.attn_kv_heads, c.head_dim, c.rope_dim, c.max_pos, c.eps,
+                              w.q_norm, w.k_norm, m.rope_cos, m.rope_sin};
+    if ((rc = sdb_attention(&ap, seqs, mix, n, reinterpret_cast<uint16_t*>(ws + L.q),
+                            reinterpret_cast<uint16_t*>(ws + L.k), reinterpret_cast<uint16_t*>(ws + L.v), act,
+                            L.act_lo, pool, m.kind_index[li], 0, st)))
+      return rc;
+    k_out = m.attn_o_in();
+  }
+  if ((rc = sdb::sdb_quantize_int8(act, act + L.act_lo, B200_ACT_BF16, T, k_out, k_out, aq, k_out, as, st))) return rc;
+  if ((rc = linear(aq, as, k_out, w.mix_out, B200_EP_RESID_ADD, c.hidden, x, c.hidden))) return rc;
+  if ((rc = norm(w.post_norm))) return rc;
+  if ((rc = linear(xq, xs, c.hidden, w.gate_up, B200_EP_SWIGLU, 2 * c.inter, act, c.inter))) return rc;
+  if ((rc = sdb::sdb_quantize_int8(act, nullptr, B200_ACT_BF16, T, c.inter, c.inter, aq, c.inter, as, st))) return rc;
+  return linear(aq, as, c.inter, w.down, B200_EP_RESID_ADD, c.hidden, x, c.hidden);
+}
+
+int check_qw(const b200_model& m, const b200_qweight& w, int n_min, int k, const char* what) {
   if (!w.data || w.n < n_min || w.k != k || w.n % 256 != 0) {
     std::string msg = std::string("b200_model_set_layer: bad weight ") + what;
     return sdb_fail(B200_ERR_SHAPE, msg.c_str());
+  }
+  if ((w.format == B200_W_INT8) != m.int8() || (m.int8() && !w.row_scale)) {
+    std::string msg = std::string("b200_model_set_layer: int8 weights (with row scales) belong to an int8 model: ") + what;
+    return sdb_fail(B200_ERR_FORMAT, msg.c_str());
   }
   return B200_OK;
 }
@@ -207,7 +278,10 @@ extern "C" int b200_model_create(const b200_model_config* cfg, b200_model** out)
   if (!cfg || !out) return sdb_fail(B200_ERR_ARG, "b200_model_create: null pointer");
   if (cfg->n_layers <= 0 || cfg->n_layers > 64 || cfg->hidden % 128 != 0 || cfg->inter % 128 != 0)
     return sdb_fail(B200_ERR_SHAPE, "b200_model_create: bad layer count or hidden/inter not a multiple of 128");
-  if (cfg->weight_format < 0 || cfg->weight_format > 3) return sdb_fail(B200_ERR_FORMAT, "b200_model_create: format");
+  if (cfg->weight_format < 0 || cfg->weight_format > B200_W_INT8)
+    return sdb_fail(B200_ERR_FORMAT, "b200_model_create: format");
+  if (cfg->weight_format == B200_W_INT8 && !(cfg->eps > 0.0f))
+    return sdb_fail(B200_ERR_ARG, "b200_model_create: an int8 model needs eps > 0");
   if (cfg->lo_format != B200_LO_BF16 && cfg->lo_format != B200_LO_E4M3)
     return sdb_fail(B200_ERR_ARG, "b200_model_create: unknown lo_format");
   auto* m = new b200_model();
@@ -245,17 +319,17 @@ extern "C" int b200_model_set_layer(b200_model* m, int32_t layer, const b200_lay
   const bool gdn = c.layer_kind[layer] == B200_LAYER_GDN;
   int rc;
   if (gdn) {
-    if ((rc = check_qw(w->mix_in, m->gdn_split() + 2 * c.gdn_heads, c.hidden, "mix_in"))) return rc;
-    if ((rc = check_qw(w->mix_out, c.hidden, m->value_dim(), "mix_out"))) return rc;
+    if ((rc = check_qw(*m, w->mix_in, m->gdn_split() + 2 * c.gdn_heads, c.hidden, "mix_in"))) return rc;
+    if ((rc = check_qw(*m, w->mix_out, c.hidden, m->value_dim(), "mix_out"))) return rc;
     if (!w->gdn.conv_w || !w->gdn.a_log || !w->gdn.dt_bias || !w->gdn.norm_w)
       return sdb_fail(B200_ERR_ARG, "b200_model_set_layer: null GDN parameter");
   } else {
-    if ((rc = check_qw(w->mix_in, m->attn_qkv(), c.hidden, "mix_in"))) return rc;
-    if ((rc = check_qw(w->mix_out, c.hidden, m->attn_o_in(), "mix_out"))) return rc;
+    if ((rc = check_qw(*m, w->mix_in, m->attn_qkv(), c.hidden, "mix_in"))) return rc;
+    if ((rc = check_qw(*m, w->mix_out, c.hidden, m->attn_o_in(), "mix_out"))) return rc;
     if (!w->q_norm || !w->k_norm) return sdb_fail(B200_ERR_ARG, "b200_model_set_layer: null q/k norm");
   }
-  if ((rc = check_qw(w->gate_up, 2 * c.inter, c.hidden, "gate_up"))) return rc;
-  if ((rc = check_qw(w->down, c.hidden, c.inter, "down"))) return rc;
+  if ((rc = check_qw(*m, w->gate_up, 2 * c.inter, c.hidden, "gate_up"))) return rc;
+  if ((rc = check_qw(*m, w->down, c.hidden, c.inter, "down"))) return rc;
   m->layers[layer] = *w;
   if (gdn) {
     m->layers[layer].gdn.heads = c.gdn_heads;
@@ -343,6 +417,10 @@ extern "C" int b200_model_forward(b200_model* m, const int32_t* ids, const b200_
   int rc;
   if ((rc = sdb_embed_vocab(ids, T, m->embed, c.hidden, x, c.vocab, st))) return rc;
   for (int li = 0; li < c.n_layers; ++li) {
+    if (m->int8()) {
+      if ((rc = forward_layer_int8(*m, li, seqs, pool, L, ws, st))) return rc;
+      continue;
+    }
     const b200_layer_weights& w = m->layers[li];
     // A small batch's in-projection splits K and accumulates its partials into `mix`: the
     // norm before it clears `mix` and the GEMM adds into it (no clearing launch of its own).

@@ -192,6 +192,8 @@ class DecisionModel:
         lo_plane: the low activation plane of those GEMMs, "bf16" (two bf16 planes, about 16
         significant bits) or "e4m3" (e4m3 low plane against an e4m3 weight copy: 3/4 of the
         tensor work, about 12 significant bits in the low term).
+        Weights in the "int8" format run the forward W8A8 (int8 codes of every linear's input, one
+        scale per token); dequant_min_tokens and lo_plane then have no effect.
         graphs: replay one CUDA graph per shape bucket (captured on first use) instead of
         launching every kernel from the host."""
         if lo_plane not in ("bf16", "e4m3"):
