@@ -10,19 +10,21 @@
 //
 // Every row is read once: its elements stay in the registers of the threads that share it while
 // the sum, the maximum and the codes follow one another.
-#include <type_traits>
-
 #include "common.cuh"
 
 namespace sdb {
 
 constexpr int I8_K_MAX = 65536;  // also keeps b200_linear_int8's sums below 2^31
 
-// The reductions of one row over its TPR threads: a warp, or a whole block.
+// The reductions of one row over its TPR threads: a group of 8 lanes, a warp, or a whole block.
+template <int TPR>
+__device__ __forceinline__ uint32_t row_lanes() {
+  return TPR >= 32 ? 0xffffffffu : ((1u << TPR) - 1u) << (threadIdx.x & 31 & ~(TPR - 1));
+}
 template <int TPR>
 __device__ __forceinline__ double row_sum(double v, double* part) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(row_lanes<TPR>(), v, o);
   if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -34,7 +36,7 @@ __device__ __forceinline__ double row_sum(double v, double* part) {
 }
 template <int TPR>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
-  v = __reduce_max_sync(0xffffffffu, v);
+  v = __reduce_max_sync(row_lanes<TPR>(), v);
   if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -91,16 +93,21 @@ struct RowArgs {
   float eps;
 };
 
+// Rows per block of TPR threads each, and the block's threads.
+template <int TPR>
+constexpr int rows_per_block() { return TPR <= 32 ? 256 / TPR : 1; }
+template <int TPR>
+constexpr int row_threads() { return TPR * rows_per_block<TPR>(); }
 template <int TPR>
 __device__ __forceinline__ int row_of() {
-  return TPR == 32 ? int(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : int(blockIdx.x);
+  return int(blockIdx.x) * rows_per_block<TPR>() + int(threadIdx.x) / TPR;
 }
 
 // TPR threads per row, NV float4 per thread (k <= 4 TPR NV).
 template <int TPR, int NV, int DELTA>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_int8_kernel(const RowArgs a) {
-  __shared__ double psum[TPR / 32];
-  __shared__ uint32_t pmax[TPR / 32];
+__global__ void __launch_bounds__(row_threads<TPR>()) rmsnorm_int8_kernel(const RowArgs a) {
+  __shared__ double psum[TPR > 32 ? TPR / 32 : 1];
+  __shared__ uint32_t pmax[TPR > 32 ? TPR / 32 : 1];
   pdl_wait();
   pdl_trigger();
   const int row = row_of<TPR>(), t = threadIdx.x % TPR;
@@ -176,9 +183,9 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_int8_kernel(con
 
 // TPR threads per row, NV groups of 4 (fp32) or 8 (bf16) elements per thread.
 template <int TPR, int NV, int TYPE>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_int8_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(row_threads<TPR>()) quantize_int8_kernel(const RowArgs a) {
   constexpr int E = TYPE == B200_ACT_F32 ? 4 : 8;
-  __shared__ uint32_t pmax[TPR / 32];
+  __shared__ uint32_t pmax[TPR > 32 ? TPR / 32 : 1];
   pdl_wait();
   pdl_trigger();
   const int row = row_of<TPR>(), t = threadIdx.x % TPR;
@@ -241,53 +248,55 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_int8_kernel(co
   }
 }
 
-// Threads per row (32: eight rows to a block of 256 threads; else a block per row) and 16-byte
-// groups per thread, for `units` groups a row: the fewest threads that hold the row in 16 groups
-// each (a warp's reductions need no barrier, and its loads are all in flight at once), but four
-// times as many while the device has under 512 threads per SM and the row has work for them.
+// Threads per row and 16-byte groups per thread, for `units` groups a row. The fewest threads that
+// hold the row in `cap` groups each: a warp's reductions need no barrier and all of its loads are
+// in flight at once, but a row that comes in two arrays fills the registers sooner (planes at 12288
+// x 2048: 19.5 us with 128 threads a row, 22.1 with 32; an fp32 delta at 12288 x 2048: 50.6 against
+// 59.2; no delta at 65536 x 2048: 116 us with 32, 123 with 128). Four times as many while the
+// device has under 512 threads per SM and the row has work for them (1 x 2048: 2.1 us against 2.5).
+// Rows of at most 32 groups take 8 lanes, four rows to a warp.
 struct RowShape {
   int tpr, nv;
 };
-static RowShape row_shape(int rows, int units) {
-  int tpr = 32;
-  while (tpr < 512 && (units > 16 * tpr || (int64_t(rows) * tpr < 512 * int64_t(sm_count()) && units > tpr))) tpr *= 4;
+static RowShape row_shape(int rows, int units, int cap) {
+  int tpr = units <= 32 ? 8 : 32;
+  while (tpr < 512 && (units > cap * tpr || (int64_t(rows) * tpr < 512 * int64_t(sm_count()) && units > tpr))) tpr *= 4;
   if (units > 16 * tpr) tpr = 1024;
   int nv = 1;
   while (nv * tpr < units) nv *= 2;
   return {tpr, nv};
 }
 
-template <int DELTA, int TPR, int NV>
-static int launch_norm(const RowArgs& a, cudaStream_t st) {
-  const int rpb = TPR == 32 ? 8 : 1;
-  SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<TPR, NV, DELTA>, dim3((a.rows + rpb - 1) / rpb), dim3(rpb * TPR), 0, st, a));
-  return B200_OK;
-}
-template <int TYPE, int TPR, int NV>
-static int launch_quant(const RowArgs& a, cudaStream_t st) {
-  const int rpb = TPR == 32 ? 8 : 1;
-  SDB_CUDA(launch_pdl(quantize_int8_kernel<TPR, NV, TYPE>, dim3((a.rows + rpb - 1) / rpb), dim3(rpb * TPR), 0, st, a));
+template <int KIND, int TPR, int NV, bool NORM>
+static int launch_row_kernel(const RowArgs& a, cudaStream_t st) {
+  constexpr int rpb = rows_per_block<TPR>();
+  const dim3 grid((a.rows + rpb - 1) / rpb), block(row_threads<TPR>());
+  if constexpr (NORM) SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<TPR, NV, KIND>, grid, block, 0, st, a));
+  else SDB_CUDA(launch_pdl(quantize_int8_kernel<TPR, NV, KIND>, grid, block, 0, st, a));
   return B200_OK;
 }
 template <bool NORM, int KIND, int TPR>
 static int launch_nv(const RowArgs& a, int nv, cudaStream_t st) {
-  auto go = [&](auto n) {
-    if constexpr (NORM) return launch_norm<KIND, TPR, decltype(n)::value>(a, st);
-    else return launch_quant<KIND, TPR, decltype(n)::value>(a, st);
-  };
-  if constexpr (TPR == 1024) return go(std::integral_constant<int, 16>{});  // only rows no block of 512 holds
-  switch (nv) {
-    case 1: return go(std::integral_constant<int, 1>{});
-    case 2: return go(std::integral_constant<int, 2>{});
-    case 4: return go(std::integral_constant<int, 4>{});
-    case 8: return go(std::integral_constant<int, 8>{});
-    default: return go(std::integral_constant<int, 16>{});
+  if constexpr (TPR == 1024) {  // only rows that no block of 512 holds
+    return launch_row_kernel<KIND, TPR, 16, NORM>(a, st);
+  } else {
+    switch (nv) {
+      case 1: return launch_row_kernel<KIND, TPR, 1, NORM>(a, st);
+      case 2: return launch_row_kernel<KIND, TPR, 2, NORM>(a, st);
+      case 4: return launch_row_kernel<KIND, TPR, 4, NORM>(a, st);
+      default: break;
+    }
+    if constexpr (TPR > 8) return nv == 8 ? launch_row_kernel<KIND, TPR, 8, NORM>(a, st)
+                                          : launch_row_kernel<KIND, TPR, 16, NORM>(a, st);
+    else return sdb_fail(B200_ERR_SHAPE, "int8 rows: no such shape");  // 8 lanes hold at most 32 groups
   }
 }
 template <bool NORM, int KIND>
 static int launch_rows(const RowArgs& a, cudaStream_t st) {
-  const RowShape r = row_shape(a.rows, a.k / (NORM || KIND == B200_ACT_F32 ? 4 : 8));
+  constexpr int cap = NORM ? (KIND == ACT_NONE ? 16 : 8) : (KIND == ACT_PLANES ? 4 : 16);
+  const RowShape r = row_shape(a.rows, a.k / (NORM || KIND == B200_ACT_F32 ? 4 : 8), cap);
   switch (r.tpr) {
+    case 8: return launch_nv<NORM, KIND, 8>(a, r.nv, st);
     case 32: return launch_nv<NORM, KIND, 32>(a, r.nv, st);
     case 128: return launch_nv<NORM, KIND, 128>(a, r.nv, st);
     case 512: return launch_nv<NORM, KIND, 512>(a, r.nv, st);
