@@ -443,8 +443,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 // memory ([token][feature], where its operands were), and after one cluster barrier CTA r adds the
 // cluster's sums of tokens r * bt / SPLIT .. and finishes them. No partial sum reaches global
 // memory and none is added atomically.
-//   warp 0  TMA ring; warp 1  MMAs; then all 8 warps drain the accumulator and finish outputs.
-constexpr int I8S_THREADS = 256;
+//   warp 0  TMA ring; warp 1  MMAs; then all warps drain the accumulator and finish outputs.
+// Warps per CTA. Alone on its SM a CTA takes 16 (1021 x 2048 x 2048: 11.5 us against 12.4); CTAs of
+// a cluster take 8, and the next launch's clusters find room beside them (128 x 2048 x 2048 on
+// clusters of 8: 8.8 us against 17.1).
+constexpr int i8s_warps(int split) { return split == 1 ? 16 : 8; }
 constexpr int I8S_OP_W = 128 * I8_BK;
 constexpr int I8S_MAX_STAGES = 12;
 constexpr int I8S_RING = 220 * 1024;       // bytes of stages: one CTA per SM
@@ -463,11 +466,12 @@ __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
 __device__ __forceinline__ int4 add4(int4 a, int4 b) { return make_int4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
 template <int EP, bool LO, int SPLIT>
-__global__ void __launch_bounds__(I8S_THREADS, 1)
+__global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
     gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                          const I8Args a) {
   extern __shared__ uint8_t i8_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int W = i8s_warps(SPLIT);
   const int bt = a.bt, stages = a.stages, x_op = bt * I8_BK;
   uint8_t* sW = smem;
   uint8_t* sX = sW + stages * I8S_OP_W;
@@ -555,7 +559,7 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
     if constexpr (EP == B200_EP_RESID_ADD) {
 #pragma unroll
       for (int i = 0; i < TB; ++i) {
-        const int c = cb + 8 * i;
+        const int c = cb + W * i;
         const float* p = static_cast<const float*>(a.o.out) + size_t(t0 + c) * a.o.ldo + f;
         r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (c < c_end && f < a.o.n_valid) {
@@ -578,7 +582,7 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
 
   // ---- sums to shared memory: warp -> lane quarter warp % 4, every second 16 tokens
   const int q = warp & 3;
-  for (int c = 16 * (warp >> 2); c < bt; c += 32) {
+  for (int c = 16 * (warp >> 2); c < bt; c += 4 * W) {
     uint32_t v[16];
     tmem_ld(tmem + c + (uint32_t(q * 32) << 16), v);
     tmem_ld_wait_for(v);
@@ -593,12 +597,12 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
   // four features per lane: 16-byte reads of each CTA's sums (4-byte ones through distributed
   // shared memory took the most of the kernel) and 16-byte stores where the output is aligned.
   const uint32_t base = smem_addr(sP);
-  for (int cb = c0 + warp; cb < c_end; cb += 8 * TB) {
+  for (int cb = c0 + warp; cb < c_end; cb += W * TB) {
     if (cb != c0 + warp) residual(cb);
     int4 v[TB], part[TB][SPLIT];
 #pragma unroll
     for (int i = 0; i < TB; ++i) {
-      const int c = min(cb + 8 * i, c_end - 1);
+      const int c = min(cb + W * i, c_end - 1);
 #pragma unroll
       for (int s = 0; s < SPLIT; ++s) {
         if constexpr (SPLIT == 1) part[i][s] = *reinterpret_cast<const int4*>(sP + c * 128 + 4 * lane);
@@ -613,7 +617,7 @@ __global__ void __launch_bounds__(I8S_THREADS, 1)
     }
 #pragma unroll
     for (int i = 0; i < TB; ++i) {
-      const int c = cb + 8 * i;
+      const int c = cb + W * i;
       if (c >= c_end) break;  // the whole warp
       const float xs = sxs[c];
       float y[4] = {i8_value(v[i].x, xs, ws[0]), i8_value(v[i].y, xs, ws[1]), i8_value(v[i].z, xs, ws[2]),
@@ -876,7 +880,7 @@ static int launch_i8_cluster(const I8Args& a, int n_tiles, int m_tiles, cudaStre
   if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, a.bt)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(SPLIT * n_tiles, m_tiles);
-  cfg.blockDim = dim3(I8S_THREADS);
+  cfg.blockDim = dim3(32 * i8s_warps(SPLIT));
   cfg.dynamicSmemBytes = i8s_smem(a.stages, a.bt);
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -898,9 +902,11 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   a.bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
   m_tiles = (a.m + a.bt - 1) / a.bt;
   const int tiles = n_tiles * m_tiles;
-  // K split over a cluster while that leaves SMs idle otherwise and every CTA two k-blocks
+  // K split over a cluster while SMs would idle and every CTA has two k-blocks. Clusters of 8 only
+  // for at most 32 tokens: they wait longest for their SMs, and each of their CTAs reads as many sums
+  // as one of 4 (2048 x 6144: 32 tokens 7.8 us against 9.2 on clusters of 4, 128 tokens 16.1 : 10.1).
   int split = 1;
-  while (split < 8 && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
+  while (split < (a.bt <= 32 ? 8 : 4) && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
   // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 200 x
   // 12288 x 2048 22.3 -> 15.5 us), or when that ring holds most of the CTA's K anyway (the next
   // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 13.4 -> 7.3 us); else the deeper
@@ -945,10 +951,12 @@ template <int EP>
 static int launch_int8(const I8Args& a, cudaStream_t st) {
   if (a.m <= 8) return dispatch_i8_reg<EP, 1>(a, st);
   if (a.m <= I8R_MAX_M) return dispatch_i8_reg<EP, 2>(a, st);
-  // pairs once every pair has a whole tile
-  const int64_t units = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
+  // Single CTAs while their 128 x 128 tiles all run at once, two to an SM (300 x 12288 x 2048: 13 us
+  // against 19 on pairs, two rounds of them); pairs beyond (512 x 12288 x 2048: 20 us against 22).
+  // (Pairs with tiles of 128 tokens, to even out their rounds, were slower: 0.8 of the time of 256.)
+  const int64_t tiles = int64_t((a.o.n_valid + 127) / 128) * ((a.m + 127) / 128);
   constexpr bool SW = EP == B200_EP_SWIGLU;
-  if (units < sm_count() / 2) {
+  if (tiles <= 2 * sm_count()) {
     if constexpr (SW) {
       if (a.o.lo_offset) return launch_i8_split<EP, true>(a, st);
     }
