@@ -115,6 +115,15 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, i
                : "memory");
 }
 
+// 5-D form of tma_load_2d_pair_hint, from the start of dimensions 1 to 3 (the SwiGLU's weight tile).
+__device__ __forceinline__ void tma_load_5d_pair_hint(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x,
+                                                      int v, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+      "[%1, {%3, %4, %4, %4, %5}], [%2], %6;" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(0), "r"(v), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -138,26 +147,21 @@ __device__ __forceinline__ void tma_store_wait_done() { asm volatile("cp.async.b
 //               (128 tokens, 32 at a time; the next ones leave TMEM while these are finished)
 constexpr int I8P_THREADS = 320;
 constexpr int I8P_EPI_WARPS = 8;
-constexpr int I8P_XCH_LD = 20;  // floats per lane of an exchange buffer (16 tokens; 16-byte accesses
-                                // of 8 neighbouring lanes then fall into different banks)
-
-// How the pair kernel writes: from registers (any alignment), the SwiGLU with a low plane, or 16
-// tokens x 32 features at a time from shared memory by TMA (16-byte aligned rows: stores of 4
-// bytes, or 2 of the SwiGLU, and their addresses were the longest part of the epilogue).
+// How the pair kernel writes: from registers (any alignment), the SwiGLU with a low plane, or 32
+// features x 16 tokens (the SwiGLU: 16 x 32) at a time from shared memory by TMA (16-byte aligned
+// rows: stores of 4 or 2 bytes and their addresses were the longest part of the epilogue).
 enum I8Out { I8_DIRECT = 0, I8_PLANES = 1, I8_TMA = 2 };
 
 template <int EP, int OUT>
 struct I8PairSmem {
   static constexpr int OP = 128 * I8_BK;                    // one operand of a stage
   static constexpr int STAGE = 2 * OP;
-  // one stage goes to the tiles of TMA stores, or to the SwiGLU's exchange of gate and up sums
-  // between lane halves: [round parity][token half, feature half][side][lane][16 tokens]
-  static constexpr int STAGES = EP == B200_EP_SWIGLU || OUT == I8_TMA ? 5 : 6;
+  // the fp32 tiles of TMA stores take a stage's room
+  static constexpr int STAGES = EP == B200_EP_STORE && OUT == I8_TMA ? 5 : 6;
   static constexpr int OT = OUT == I8_TMA ? 16 * 32 * (EP == B200_EP_SWIGLU ? 2 : 4) : 0;  // one tile of a store
-  static constexpr int XCH = EP == B200_EP_SWIGLU ? 2 * 4 * 2 * 32 * I8P_XCH_LD * 4 : 0;
   static constexpr int XS = I8P_EPI_WARPS * 128 * 4;        // each epilogue warp's token scales
   static constexpr int BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = 1024 + STAGES * STAGE + 2 * I8P_EPI_WARPS * OT + XCH + XS + BARS * 8 + 16;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE + 2 * I8P_EPI_WARPS * OT + XS + BARS * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -189,8 +193,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   uint8_t* sW = smem;
   uint8_t* sX = sW + SM::STAGES * SM::OP;
   uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp][2] tiles of TMA stores
-  float* xch = reinterpret_cast<float*>(sO + 2 * I8P_EPI_WARPS * SM::OT);
-  float* sxs = xch + SM::XCH / 4;
+  float* sxs = reinterpret_cast<float*>(sO + 2 * I8P_EPI_WARPS * SM::OT);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxs + SM::XS / 4);
   uint64_t* full = bars;                            // the leader's are used
   uint64_t* empty = bars + SM::STAGES;              // both CTAs'
@@ -252,7 +255,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
           mbar_wait(&empty[s], ph ^ 1, FAULT_GEMM_WAIT_EMPTY);
           const uint32_t fb = full0 + 8u * s;
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * SM::STAGE);
-          tma_load_2d_pair_hint(sW + s * SM::OP, &tmW, fb, kt * (I8_BK / 2), n0, keep);
+          if constexpr (EP == B200_EP_SWIGLU)
+            tma_load_5d_pair_hint(sW + s * SM::OP, &tmW, fb, kt * (I8_BK / 2), n0 / 128, keep);
+          else
+            tma_load_2d_pair_hint(sW + s * SM::OP, &tmW, fb, kt * (I8_BK / 2), n0, keep);
           tma_load_2d_pair(sX + s * SM::OP, &tmX, fb, kt * (I8_BK / 2), t0);
           if (++s == SM::STAGES) s = 0, ph ^= 1;
         }
@@ -302,76 +308,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       __syncwarp();
       if (lane == 0) tma_store_2d(&tmO, tiles + which * SM::OT, x, y);
     };
+    // this lane's feature of a tile: its row, or in the SwiGLU's order of rows (i8_swiglu_map) gate
+    // feature 16 q + lane % 16 in the lower lanes and the matching up feature in the upper ones
+    const bool up = lane >= 16;
+    const int row = EP == B200_EP_SWIGLU ? 16 * q + (lane & 15) + (up ? 64 : 0) : 32 * q + lane;
+    // the channel scale and token scales of a unit, read while the unit before is finished
+    float ws_next = 0.0f, xs_next[4] = {};
+    auto scales = [&](int u) {
+      int mt, nt;
+      tile_of(u, mt, nt);
+      const int n = nt * 256 + int(rank) * 128 + row, t0 = mt * 256 + 128 * hf;
+      ws_next = n < a.n ? a.ws[n] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xs_next[i] = t0 + 32 * i + lane < a.m ? a.xs[t0 + 32 * i + lane] : 0.0f;
+    };
+    if (pair < n_units) scales(pair);
     uint32_t local = 0;
     for (int u = pair; u < n_units; u += n_pairs, ++local) {
       int mt, nt;
       tile_of(u, mt, nt);
-      const int n0 = nt * 256 + int(rank) * 128, n = n0 + 32 * q + lane;
+      const int n0 = nt * 256 + int(rank) * 128, n = n0 + row;
       const int t0 = mt * 256 + 128 * hf, left = a.m - t0;  // this warp's first token, tokens from it on
-      const float ws = n < a.n ? a.ws[n] : 0.0f;
       const uint32_t ab = local & 1, aph = (local >> 1) & 1;
       const uint32_t tl = tmem + ab * 256 + 128 * hf + (uint32_t(q * 32) << 16);
-      float xv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xv[i] = 32 * i + lane < left ? a.xs[t0 + 32 * i + lane] : 0.0f;
+      const float ws = ws_next;
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xs[32 * i + lane] = xv[i];
+      for (int i = 0; i < 4; ++i) xs[32 * i + lane] = xs_next[i];
       __syncwarp();
+      if (u + n_pairs < n_units) scales(u + n_pairs);
       if constexpr (EP == B200_EP_SWIGLU) {
-        // Lanes 0..63 of the tile hold gate features, 64..127 the up features of the same outputs:
-        // of every 32 tokens warps q and q ^ 2 finish 16 each and send the other 16. Two buffers by
-        // round parity: a warp reaches a round's barrier only after it has read the round before.
-        const int side = q >> 1, grp = hf * 2 + (q & 1);
-        const int sc = side ? 0 : 16, oc = side ? 16 : 0;  // columns sent, columns finished
-        float* mine = xch + ((grp * 2 + side) * 32 + lane) * I8P_XCH_LD;
-        const float* theirs = xch + ((grp * 2 + (side ^ 1)) * 32 + lane) * I8P_XCH_LD;
-        constexpr int XB = 4 * 2 * 32 * I8P_XCH_LD;  // floats of one parity's buffers
+        // of two tokens the gate lane finishes the first and its up lane the second: each sends the
+        // other the value it lacks
         const bool valid = n0 < a.o.n_valid;
-        const size_t idx0 = size_t(t0 + oc) * a.o.ldo + n0 / 2 + 32 * (q & 1) + lane;
-        uint32_t vs[2][16], vo[2][16];
+        const size_t idx0 = size_t(t0 + (up ? 1 : 0)) * a.o.ldo + n0 / 2 + 16 * q + (lane & 15);
+        uint32_t v[2][32];
         mbar_wait(&acc_full[ab], aph, FAULT_GEMM_WAIT_ACCUM);
         tc_fence_after();
-        tmem_ld(tl + sc, vs[0]);
-        tmem_ld(tl + oc, vo[0]);
+        tmem_ld(tl, v[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait_for(vs[c & 1]);
-          tmem_ld_wait_for(vo[c & 1]);
-          if (c < 3) {
-            tmem_ld(tl + 32 * (c + 1) + sc, vs[(c + 1) & 1]);
-            tmem_ld(tl + 32 * (c + 1) + oc, vo[(c + 1) & 1]);
-          }
-          const float* xc = xs + 32 * c;
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(xc + sc + j);
-            *reinterpret_cast<float4*>(mine + (c & 1) * XB + j) =
-                make_float4(i8_value(int(vs[c & 1][j]), x.x, ws), i8_value(int(vs[c & 1][j + 1]), x.y, ws),
-                            i8_value(int(vs[c & 1][j + 2]), x.z, ws), i8_value(int(vs[c & 1][j + 3]), x.w, ws));
-          }
+          tmem_ld_wait_for(v[c & 1]);
+          if (c < 3) tmem_ld(tl + 32 * (c + 1), v[(c + 1) & 1]);
+          const int l = left - 32 * c;
+          const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
+          uint16_t* tile = reinterpret_cast<uint16_t*>(tiles + (c & 1) * SM::OT) + lane;
           tile_free();
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + grp) : "memory");
-          if (valid) {
-            const int l = left - 32 * c - oc;  // of these 16 tokens, the ones inside the batch
-            const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
-            uint16_t* tile = reinterpret_cast<uint16_t*>(tiles + (c & 1) * SM::OT) + lane;
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(xc + oc + j);
-              const float4 o4 = *reinterpret_cast<const float4*>(theirs + (c & 1) * XB + j);
-              const float xe[4] = {x.x, x.y, x.z, x.w}, oe[4] = {o4.x, o4.y, o4.z, o4.w};
+          for (int j = 0; j < 32; j += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(xs + 32 * c + j);
+            const float xe[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float own = i8_value(int(vo[c & 1][j + e]), xe[e], ws);
-                const float gv = side ? oe[e] : own, uv = side ? own : oe[e];
-                if constexpr (OUT == I8_TMA) tile[32 * (j + e)] = f32_to_bf16_rn(swiglu(gv, uv));
-                else if (j + e < l) store_swiglu<OUT == I8_PLANES>(a.o, idx + size_t(j + e) * a.o.ldo, gv, uv);
-              }
+            for (int e = 0; e < 4; e += 2) {
+              const float y0 = i8_value(int(v[c & 1][j + e]), xe[e], ws);
+              const float y1 = i8_value(int(v[c & 1][j + e + 1]), xe[e + 1], ws);
+              const float other = __shfl_xor_sync(0xffffffffu, up ? y0 : y1, 16);
+              const float g = up ? other : y0, uv = up ? y1 : other;
+              if constexpr (OUT == I8_TMA) tile[16 * (j + e)] = f32_to_bf16_rn(swiglu(g, uv));
+              else if (valid && j + e + (up ? 1 : 0) < l)
+                store_swiglu<OUT == I8_PLANES>(a.o, idx + size_t(j + e) * a.o.ldo, g, uv);
             }
-            if constexpr (OUT == I8_TMA) {
-              if (l > 0) tile_store(c & 1, n0 / 2 + 32 * (q & 1), t0 + 32 * c + oc);
-            }
+          }
+          if constexpr (OUT == I8_TMA) {
+            if (valid && l > 0) tile_store(c & 1, n0 / 2 + 16 * q, t0 + 32 * c);
           }
         }
       } else {
@@ -824,6 +823,17 @@ static int i8_map(CUtensorMap* map, const void* base, int rows, int k, int ld, i
   return encode_bf16_sw128(map, base, 2, dims, strides, box);
 }
 
+// The pair kernel's SwiGLU weight tile: a block's 64 gate and 64 up rows in the order 16 gate, the
+// matching 16 up, the next 16 gate, ..., so that a warp's 32 accumulator lanes hold both values of
+// its 16 outputs. Dimensions: code, row of 16, gate / up, 16s of the 64, block of 128 rows.
+static int i8_swiglu_map(CUtensorMap* map, const void* base, int blocks, int k) {
+  const uint64_t kk = uint64_t(k);
+  const uint64_t dims[5] = {kk / 2, 16, 2, 4, uint64_t(blocks)};
+  const uint64_t strides[4] = {kk, 64 * kk, 16 * kk, 128 * kk};
+  const uint32_t box[5] = {I8_BK / 2, 16, 2, 4, 1};
+  return encode_bf16_sw128(map, base, 5, dims, strides, box);
+}
+
 template <int EP, int OUT>
 static int launch_i8_pair(I8Args a, cudaStream_t st) {
   constexpr int smem = I8PairSmem<EP, OUT>::TOTAL;
@@ -847,12 +857,13 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   int dev = 0;
   SDB_CUDA(cudaGetDevice(&dev));
   CUtensorMap mw, mx, mo;
-  if (int rc = i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
-  if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, 128)) return rc;
   constexpr bool SW = EP == B200_EP_SWIGLU;
+  if (int rc = SW ? i8_swiglu_map(&mw, a.w, a.o.n_valid / 128, a.k) : i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
+  if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, 128)) return rc;
   mo = mw;  // not read
   if constexpr (OUT == I8_TMA) {
-    if (int rc = encode_store_tile(&mo, a.o.out, SW ? 2 : 4, a.m, SW ? a.o.n_valid / 2 : a.o.n_valid, a.o.ldo, 16, 32))
+    if (int rc = encode_store_tile(&mo, a.o.out, SW ? 2 : 4, a.m, SW ? a.o.n_valid / 2 : a.o.n_valid, a.o.ldo, SW ? 32 : 16,
+                                   SW ? 16 : 32))
       return rc;
   }
   const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + 255) / 256;
