@@ -196,7 +196,7 @@ enum b200_act_type { B200_ACT_F32 = 0, B200_ACT_BF16 = 1 };
 
 /* Int8 codes q [rows, ldq] and scales [rows] of x [rows, ldx] (fp32, or bf16 bit patterns). With
  * x_lo (bf16 only, same ldx) the row is v = fl(x + x_lo): the two planes the mixers and the SwiGLU
- * epilogue write. k a multiple of 16, at most 65536; ldx in elements, ldx * element size and ldq
+ * epilogue write. k a multiple of 16, at most 65536; at most 2^30 rows; ldx in elements, ldx * element size and ldq
  * multiples of 16; x, x_lo and q 16-byte aligned. Columns k .. ldq - 1 of q are left as they
  * were. */
 int b200_quantize_act_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t rows, int32_t k, int32_t ldx,
@@ -207,15 +207,15 @@ int b200_quantize_act_int8(const void* x, const uint16_t* x_lo, int32_t type, in
  *   v = fl(fl(t * r) * fl(1 + w)); q, scale = the codes of v.
  * x fp32 [rows, ldx]; delta (optional) fp32 or bf16 [rows, ldd]; sum (optional, needs delta)
  * receives t as fp32 [rows, lds] and may be x or an fp32 delta themselves (same stride), with no
- * other overlap. hidden a multiple of 16, at most 65536; every row stride in bytes a multiple of
+ * other overlap. hidden a multiple of 16, at most 65536; at most 2^30 rows; every row stride in bytes a multiple of
  * 16 and every pointer 16-byte aligned; eps > 0. */
 int b200_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t delta_type, int32_t ldd, float* sum,
                       int32_t lds, int32_t rows, int32_t hidden, const float* w, float eps, int8_t* q, int32_t ldq,
                       float* scale, b200_stream stream);
 
 /* The product above with b200_linear's epilogues, for q [m, ldx] codes (any int8 values, from
- * either call above or the caller's own), x_scale [m] and a B200_W_INT8 weight. Any m >= 1 and any
- * w->n; k = w->k a multiple of 16, at most 65536; ldx a multiple of 16; q and w->data 16-byte
+ * either call above or the caller's own), x_scale [m] and a B200_W_INT8 weight. Any m and w->n from 1
+ * to 2^30; k = w->k a multiple of 16, at most 65536; ldx a multiple of 16; q and w->data 16-byte
  * aligned. Only columns < n_valid are written: any n_valid <= w->n for STORE and RESID_ADD; a
  * multiple of 128 for SWIGLU, whose weight rows are interleaved in blocks of 64 (gate, up). The
  * SwiGLU's lo plane follows lo_offset and lo_format as in b200_linear. ldo: any that holds a row.

@@ -1077,6 +1077,7 @@ int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64
 int encode_store_tile(CUtensorMap* map, const void* base, int elem_bytes, int rows, int cols, int64_t ld,
                       int box_rows, int box_cols) {
   if (int rc = get_encode_fn()) return rc;
+  if (int64_t(cols) * elem_bytes % 16 != 0) return sdb_fail(B200_ERR_SHAPE, "encode_store_tile: cols end inside 16 bytes");
   const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
   const cuuint64_t strides[1] = {cuuint64_t(ld) * elem_bytes};
   const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};

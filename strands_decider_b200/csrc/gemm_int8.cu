@@ -149,19 +149,21 @@ constexpr int I8P_THREADS = 320;
 constexpr int I8P_EPI_WARPS = 8;
 // How the pair kernel writes: from registers (any alignment), the SwiGLU with a low plane, or 32
 // features x 16 tokens (the SwiGLU: 16 x 32) at a time from shared memory by TMA (16-byte aligned
-// rows: stores of 4 or 2 bytes and their addresses were the longest part of the epilogue).
+// rows: stores of 4 or 2 bytes and their addresses were the longest part of the epilogue). With a
+// residual the tile is loaded by TMA two tiles ahead, added to where it lies, and stored.
 enum I8Out { I8_DIRECT = 0, I8_PLANES = 1, I8_TMA = 2 };
 
 template <int EP, int OUT>
 struct I8PairSmem {
   static constexpr int OP = 128 * I8_BK;                    // one operand of a stage
   static constexpr int STAGE = 2 * OP;
-  // the fp32 tiles of TMA stores take a stage's room
-  static constexpr int STAGES = EP == B200_EP_STORE && OUT == I8_TMA ? 5 : 6;
+  // the fp32 tiles of TMA stores take a stage's room, those of a residual two
+  static constexpr int STAGES = OUT != I8_TMA || EP == B200_EP_SWIGLU ? 6 : EP == B200_EP_STORE ? 5 : 4;
   static constexpr int OT = OUT == I8_TMA ? 16 * 32 * (EP == B200_EP_SWIGLU ? 2 : 4) : 0;  // one tile of a store
+  static constexpr int OTS = EP == B200_EP_RESID_ADD ? 4 : 2;                              // tiles per epilogue warp
   static constexpr int XS = I8P_EPI_WARPS * 128 * 4;        // each epilogue warp's token scales
-  static constexpr int BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = 1024 + STAGES * STAGE + 2 * I8P_EPI_WARPS * OT + XS + BARS * 8 + 16;
+  static constexpr int BARS = 2 * STAGES + 4 + 4 * I8P_EPI_WARPS;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE + OTS * I8P_EPI_WARPS * OT + XS + BARS * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -193,12 +195,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   uint8_t* sW = smem;
   uint8_t* sX = sW + SM::STAGES * SM::OP;
   uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp][2] tiles of TMA stores
-  float* sxs = reinterpret_cast<float*>(sO + 2 * I8P_EPI_WARPS * SM::OT);
+  float* sxs = reinterpret_cast<float*>(sO + SM::OTS * I8P_EPI_WARPS * SM::OT);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxs + SM::XS / 4);
   uint64_t* full = bars;                            // the leader's are used
   uint64_t* empty = bars + SM::STAGES;              // both CTAs'
   uint64_t* acc_full = bars + 2 * SM::STAGES;       // [2], both CTAs'
   uint64_t* acc_empty = bars + 2 * SM::STAGES + 2;  // [2], the leader's are used
+  uint64_t* res_full = bars + 2 * SM::STAGES + 4;   // [epilogue warp][4]: a residual tile has landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SM::BARS);
 
   const uint32_t rank = cluster_ctarank();
@@ -226,6 +229,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2 * I8P_EPI_WARPS);
     }
+    for (int b = 0; b < 4 * I8P_EPI_WARPS; ++b) mbar_init(&res_full[b], 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -296,17 +300,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     const int q = warp & 3, hf = (warp - 2) >> 2;
     const uint32_t acc_empty0 = mapa_shared(smem_addr(acc_empty), 0);
     float* xs = sxs + (warp - 2) * 128;  // scales of this warp's 128 tokens
-    uint8_t* tiles = sO + 2 * (warp - 2) * SM::OT;
-    auto tile_free = [&]() {  // the tile about to be filled was read by its last store
-      if constexpr (OUT == I8_TMA) {
-        if (lane == 0) tma_store_wait_read<1>();
-        __syncwarp();
-      }
+    uint8_t* tiles = sO + SM::OTS * (warp - 2) * SM::OT;
+    // Store tiles: the g-th tile that this warp stores (tiles with nothing to store are left out, and
+    // not written either) lies in buffer g % 2, free once the store before the last has read it.
+    uint32_t sg = 0;
+    auto tile_free = [&]() {
+      if (lane == 0) tma_store_wait_read<1>();
+      __syncwarp();
+      return tiles + (sg++ & 1) * SM::OT;
     };
-    auto tile_store = [&](int which, int x, int y) {
+    auto tile_store = [&](const void* tile, int x, int y) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) tma_store_2d(&tmO, tiles + which * SM::OT, x, y);
+      if (lane == 0) tma_store_2d(&tmO, tile, x, y);
     };
     // this lane's feature of a tile: its row, or in the SwiGLU's order of rows (i8_swiglu_map) gate
     // feature 16 q + lane % 16 in the lower lanes and the matching up feature in the upper ones
@@ -323,6 +329,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       for (int i = 0; i < 4; ++i) xs_next[i] = t0 + 32 * i + lane < a.m ? a.xs[t0 + 32 * i + lane] : 0.0f;
     };
     if (pair < n_units) scales(pair);
+    // Residual tiles: the g-th tile of this warp (over its units, empty ones left out) goes through
+    // buffer g % 4. A tile is asked for two tiles ahead, when the store of the tile that was in its
+    // buffer is the last but one.
+    int pu = pair, pc = 0;          // the next tile to ask for: unit, 16-token chunk
+    uint32_t pg = 0, rg = 0;        // tiles asked for, tiles finished
+    auto chunks = [&](int n0, int left) { return n0 + 32 * q < a.o.n_valid ? min(8, max(0, left + 15) / 16) : 0; };
+    auto ask = [&]() {
+      int n0 = 0, t0 = 0;
+      for (; pu < n_units; pu += n_pairs, pc = 0) {
+        int mt, nt;
+        tile_of(pu, mt, nt);
+        n0 = nt * 256 + int(rank) * 128, t0 = mt * 256 + 128 * hf;
+        if (pc < chunks(n0, a.m - t0)) break;
+      }
+      if (pu >= n_units) return;
+      if (lane == 0) {
+        uint64_t* bar = &res_full[4 * (warp - 2) + (pg & 3)];
+        tma_store_wait_read<1>();
+        mbar_arrive_expect_tx(bar, SM::OT);
+        tma_load_2d(tiles + (pg & 3) * SM::OT, &tmO, bar, n0 + 32 * q, t0 + 16 * pc);
+      }
+      ++pc;
+      ++pg;
+    };
+    if constexpr (EP == B200_EP_RESID_ADD && OUT == I8_TMA) {
+      ask();
+      ask();
+    }
     uint32_t local = 0;
     for (int u = pair; u < n_units; u += n_pairs, ++local) {
       int mt, nt;
@@ -352,8 +386,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
           if (c < 3) tmem_ld(tl + 32 * (c + 1), v[(c + 1) & 1]);
           const int l = left - 32 * c;
           const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
-          uint16_t* tile = reinterpret_cast<uint16_t*>(tiles + (c & 1) * SM::OT) + lane;
-          tile_free();
+          if (!valid || l <= 0) continue;  // the whole warp
+          uint8_t* tile = nullptr;
+          if constexpr (OUT == I8_TMA) tile = tile_free();
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 x = *reinterpret_cast<const float4*>(xs + 32 * c + j);
@@ -364,14 +399,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
               const float y1 = i8_value(int(v[c & 1][j + e + 1]), xe[e + 1], ws);
               const float other = __shfl_xor_sync(0xffffffffu, up ? y0 : y1, 16);
               const float g = up ? other : y0, uv = up ? y1 : other;
-              if constexpr (OUT == I8_TMA) tile[16 * (j + e)] = f32_to_bf16_rn(swiglu(g, uv));
-              else if (valid && j + e + (up ? 1 : 0) < l)
+              if constexpr (OUT == I8_TMA)
+                reinterpret_cast<uint16_t*>(tile)[16 * (j + e) + lane] = f32_to_bf16_rn(swiglu(g, uv));
+              else if (j + e + (up ? 1 : 0) < l)
                 store_swiglu<OUT == I8_PLANES>(a.o, idx + size_t(j + e) * a.o.ldo, g, uv);
             }
           }
-          if constexpr (OUT == I8_TMA) {
-            if (valid && l > 0) tile_store(c & 1, n0 / 2 + 16 * q, t0 + 32 * c);
-          }
+          if constexpr (OUT == I8_TMA) tile_store(tile, n0 / 2 + 16 * q, t0 + 32 * c);
         }
       } else {
         float* p = static_cast<float*>(a.o.out) + size_t(t0) * a.o.ldo + n;
@@ -380,7 +414,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
         constexpr int CW = EP == B200_EP_RESID_ADD || OUT == I8_TMA ? 16 : 32;
         float r[2][CW];
         auto residual = [&](int c) {  // chunk c's residual, read while the chunk before is finished
-          if constexpr (EP == B200_EP_RESID_ADD) {
+          if constexpr (EP == B200_EP_RESID_ADD && OUT == I8_DIRECT) {
 #pragma unroll
             for (int j = 0; j < CW; ++j)
               r[c & 1][j] = valid && CW * c + j < left ? p[size_t(CW * c + j) * a.o.ldo] : 0.0f;
@@ -399,18 +433,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
             residual(c + 1);
           }
           const int l = left - CW * c;
-          if constexpr (OUT == I8_TMA) {
-            tile_free();
-            float* tile = reinterpret_cast<float*>(tiles + (c & 1) * SM::OT) + lane;
+          if constexpr (OUT == I8_TMA && EP == B200_EP_RESID_ADD) {
+            if (c < chunks(n0, left)) {
+              ask();
+              mbar_wait(&res_full[4 * (warp - 2) + (rg & 3)], (rg >> 2) & 1, FAULT_GEMM_WAIT_FULL_W);
+              __syncwarp();
+              float* tile = reinterpret_cast<float*>(tiles + (rg & 3) * SM::OT) + lane;
 #pragma unroll
-            for (int j = 0; j < CW; j += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(xs + CW * c + j);
-              tile[32 * j] = i8_value(int(v[c & 1][j]), x.x, ws);
-              tile[32 * (j + 1)] = i8_value(int(v[c & 1][j + 1]), x.y, ws);
-              tile[32 * (j + 2)] = i8_value(int(v[c & 1][j + 2]), x.z, ws);
-              tile[32 * (j + 3)] = i8_value(int(v[c & 1][j + 3]), x.w, ws);
+              for (int j = 0; j < CW; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(xs + CW * c + j);
+                const float xe[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float* t = tile + 32 * (j + e);
+                  *t = __fadd_rn(*t, i8_value(int(v[c & 1][j + e]), xe[e], ws));
+                }
+              }
+              tile_store(tiles + (rg & 3) * SM::OT, n0 + 32 * q, t0 + CW * c);
+              ++rg;
             }
-            if (l > 0 && n0 + 32 * q < a.o.n_valid) tile_store(c & 1, n0 + 32 * q, t0 + CW * c);
+          } else if constexpr (OUT == I8_TMA) {
+            if (c < chunks(n0, left)) {
+              uint8_t* const dst = tile_free();
+              float* tile = reinterpret_cast<float*>(dst) + lane;
+#pragma unroll
+              for (int j = 0; j < CW; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(xs + CW * c + j);
+                tile[32 * j] = i8_value(int(v[c & 1][j]), x.x, ws);
+                tile[32 * (j + 1)] = i8_value(int(v[c & 1][j + 1]), x.y, ws);
+                tile[32 * (j + 2)] = i8_value(int(v[c & 1][j + 2]), x.z, ws);
+                tile[32 * (j + 3)] = i8_value(int(v[c & 1][j + 3]), x.w, ws);
+              }
+              tile_store(dst, n0 + 32 * q, t0 + CW * c);
+            }
           } else if (valid) {
             float* pc = p + size_t(CW * c) * a.o.ldo;
             if (l >= CW) i8_finish<EP, true>(a, v[c & 1], xs + CW * c, ws, pc, r[c & 1], l);
@@ -976,10 +1031,10 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   if constexpr (SW) {
     if (a.o.lo_offset) return launch_i8_pair<EP, I8_PLANES>(a, st);
   }
-  if constexpr (EP != B200_EP_RESID_ADD) {
-    if (int64_t(a.o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o.out) & 15) == 0)
-      return launch_i8_pair<EP, I8_TMA>(a, st);
-  }
+  // A TMA tile ends at a whole 16 bytes: with 3999 outputs it would write the 4000th column too.
+  if (int64_t(a.o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o.out) & 15) == 0 &&
+      (SW || a.o.n_valid % 4 == 0))
+    return launch_i8_pair<EP, I8_TMA>(a, st);
   return launch_i8_pair<EP, I8_DIRECT>(a, st);
 }
 
@@ -990,6 +1045,7 @@ int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k,
   if (w->format != B200_W_INT8) return sdb_fail(B200_ERR_FORMAT, "b200_linear_int8: needs a B200_W_INT8 weight");
   if (!w->row_scale) return sdb_fail(B200_ERR_ARG, "b200_linear_int8: missing row_scale");
   if (m <= 0 || k <= 0 || w->n <= 0) return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: empty shape");
+  if (m > 1 << 30 || w->n > 1 << 30) return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: more than 2^30 rows");
   if (w->k != k) return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: q and W disagree on k");
   if (k % 16 != 0 || k > 65536)
     return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: k must be a multiple of 16, at most 65536");

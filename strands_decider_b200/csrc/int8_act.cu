@@ -14,7 +14,8 @@
 
 namespace sdb {
 
-constexpr int I8_K_MAX = 65536;  // also keeps b200_linear_int8's sums below 2^31
+constexpr int I8_K_MAX = 65536;          // also keeps b200_linear_int8's sums below 2^31
+constexpr int I8_ROWS_MAX = 1 << 30;     // counts of rows and tiles then fit 32 bits after rounding up
 
 // The reductions of one row over its TPR threads: a group of 8 lanes, a warp, or a whole block.
 template <int TPR>
@@ -314,6 +315,7 @@ int sdb_quantize_int8(const void* x, const uint16_t* x_lo, int32_t type, int32_t
   if (x_lo && type != B200_ACT_BF16)
     return sdb_fail(B200_ERR_ARG, "b200_quantize_act_int8: a low plane belongs to bf16 activations");
   if (rows <= 0 || k <= 0) return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: empty shape");
+  if (rows > I8_ROWS_MAX) return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: more than 2^30 rows");
   if (k % 16 != 0 || k > I8_K_MAX)
     return sdb_fail(B200_ERR_SHAPE, "b200_quantize_act_int8: k must be a multiple of 16, at most 65536");
   if (ldx < k || ldx % (type == B200_ACT_F32 ? 4 : 8) != 0 || ldq < k || ldq % 16 != 0)
@@ -342,6 +344,7 @@ int sdb_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t del
     return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: unknown delta type");
   if (!(eps > 0.0f)) return sdb_fail(B200_ERR_ARG, "b200_rmsnorm_int8: eps must be positive");
   if (rows <= 0 || hidden <= 0) return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: empty shape");
+  if (rows > I8_ROWS_MAX) return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: more than 2^30 rows");
   if (hidden % 16 != 0 || hidden > I8_K_MAX)
     return sdb_fail(B200_ERR_SHAPE, "b200_rmsnorm_int8: hidden must be a multiple of 16, at most 65536");
   if (ldx < hidden || ldx % 4 != 0 || ldq < hidden || ldq % 16 != 0 ||

@@ -44,6 +44,7 @@ def test_quantize_act_int8(lib, p16):
     bad(1, lo=p16)                       # a low plane of fp32 activations
     bad(2, rows=0)
     bad(2, rows=-3)
+    bad(2, rows=(1 << 30) + 1)
     bad(2, k=0)
     bad(2, k=24, ldx=32, ldq=32)         # not a multiple of 16
     bad(2, k=65552, ldx=65552, ldq=65552)
@@ -75,6 +76,7 @@ def test_rmsnorm_int8(lib, p16):
     bad(1, eps=0.0)
     bad(1, eps=float("nan"))
     bad(2, rows=0)
+    bad(2, rows=(1 << 30) + 1)
     bad(2, k=0)
     bad(2, k=40, ldx=64)
     bad(2, k=65552, ldx=65552, ldd=65552, lds=65552, ldq=65552)
@@ -101,7 +103,7 @@ def test_linear_int8(lib, p16):
         bad(1, **kw)
     for fmt in (0, 1, 2, 3, 5, -1):
         bad(3, fmt=fmt)
-    for kw in (dict(m=0), dict(m=-1), dict(k=0, wk=0), dict(n=0), dict(wk=128), dict(k=40, wk=40),
+    for kw in (dict(m=0), dict(m=-1), dict(m=(1 << 30) + 1), dict(n=(1 << 30) + 1), dict(k=0, wk=0), dict(n=0), dict(wk=128), dict(k=40, wk=40),
                dict(k=65552, wk=65552, ldx=65552), dict(ldx=48), dict(ldx=72), dict(q=p16 + 8), dict(data=p16 + 4),
                dict(nv=0), dict(nv=129), dict(ldo=127), dict(out=p16 + 2), dict(ep=2, nv=64), dict(ep=2, ldo=63),
                dict(ep=2, out=p16 + 1)):
