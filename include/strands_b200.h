@@ -218,7 +218,8 @@ int b200_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t de
  * to 2^30; k = w->k a multiple of 16, at most 65536; ldx a multiple of 16; q and w->data 16-byte
  * aligned. Only columns < n_valid are written: any n_valid <= w->n for STORE and RESID_ADD; a
  * multiple of 128 for SWIGLU, whose weight rows are interleaved in blocks of 64 (gate, up). The
- * SwiGLU's lo plane follows lo_offset and lo_format as in b200_linear. ldo: any that holds a row.
+ * SwiGLU's lo plane follows lo_offset and lo_format as in b200_linear; its values below 2^-119 |up|
+ * come out as zero. ldo: any that holds a row.
  * Results do not depend on the batch a row is in, nor on timing. */
 int b200_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
                      const b200_linear_out* out, b200_stream stream);

@@ -27,7 +27,7 @@ struct I8Args {
   int m, n, k, ldx;
   int ngroup;           // pair kernel: feature tiles per group
   int bt, stages;       // split kernel: tokens per tile, ring depth
-  int vec;              // output rows take 16-byte (SwiGLU: 8-byte) accesses at every fourth output
+  int vec;              // split kernel: every fourth output of a row is aligned to four outputs
 };
 
 constexpr int I8_BK = 128;  // bytes (= codes) of K per stage: one 128-byte swizzled row
@@ -144,7 +144,13 @@ __device__ __forceinline__ void tma_store_wait_done() { asm volatile("cp.async.b
 //   warp 0      TMA ring (both CTAs; bytes signalled on the leader's full barrier)
 //   warp 1      the leader's lane 0 issues the MMAs into one of two 256-column accumulators
 //   warps 2..9  epilogue: TMEM lane quarter warp % 4, token half (warp - 2) / 4
-//               (128 tokens, 32 at a time; the next ones leave TMEM while these are finished)
+//               (128 tokens, 16 or 32 at a time; the next ones leave TMEM while these are finished)
+// 256 x 256 is the largest tile that leaves room for a second accumulator, which the next tile's
+// products need while this one is finished: the main loop alone runs at 3425-3496 Tops/s (8192 and
+// 18944 x 12288 x 2048), and with it 13 TB/s of operands cross from L2. What is lost on top is
+// the epilogue's instructions and bytes: 8192 x 12288 x 2048 SwiGLU 148 us = 2.78 Pops/s, 65536
+// tokens 1149 us; in a seconds-long run the 1000 W cap sets 1.47 GHz and 1325 us = 2.49 Pops/s.
+// 65536 x 2048 x 6144 with the residual: 602 us = 2.74 Pops/s; x 2048: 289 us = 4.2 TB/s.
 constexpr int I8P_THREADS = 320;
 constexpr int I8P_EPI_WARPS = 8;
 // How the pair kernel writes: from registers (any alignment), the SwiGLU with a low plane, or 32
@@ -194,7 +200,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = sW + SM::STAGES * SM::OP;
-  uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp][2] tiles of TMA stores
+  uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp][OTS] tiles of TMA stores
   float* sxs = reinterpret_cast<float*>(sO + SM::OTS * I8P_EPI_WARPS * SM::OT);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxs + SM::XS / 4);
   uint64_t* full = bars;                            // the leader's are used
@@ -304,7 +310,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     // Store tiles: the g-th tile that this warp stores (tiles with nothing to store are left out, and
     // not written either) lies in buffer g % 2, free once the store before the last has read it.
     uint32_t sg = 0;
-    auto tile_free = [&]() {
+    auto free_tile = [&]() {
       if (lane == 0) tma_store_wait_read<1>();
       __syncwarp();
       return tiles + (sg++ & 1) * SM::OT;
@@ -388,7 +394,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
           const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
           if (!valid || l <= 0) continue;  // the whole warp
           uint8_t* tile = nullptr;
-          if constexpr (OUT == I8_TMA) tile = tile_free();
+          if constexpr (OUT == I8_TMA) tile = free_tile();
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 x = *reinterpret_cast<const float4*>(xs + 32 * c + j);
@@ -454,7 +460,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
             }
           } else if constexpr (OUT == I8_TMA) {
             if (c < chunks(n0, left)) {
-              uint8_t* const dst = tile_free();
+              uint8_t* const dst = free_tile();
               float* tile = reinterpret_cast<float*>(dst) + lane;
 #pragma unroll
               for (int j = 0; j < CW; j += 4) {
@@ -498,6 +504,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 // cluster's sums of tokens r * bt / SPLIT .. and finishes them. No partial sum reaches global
 // memory and none is added atomically.
 //   warp 0  TMA ring; warp 1  MMAs; then all warps drain the accumulator and finish outputs.
+// At these sizes a launch is a chain of latencies. 96 x 8224 x 2048 (clusters of 2), 9.0 us in a row
+// of launches, of which one takes 7.8: 0.5 set-up, 3.7 until the last MMA (8 k-blocks of 28 KB),
+// 0.4 sums to shared memory, 0.7 cluster barrier, 1.3 outputs, 0.8 last barrier. 1021 x 2048 x 2048,
+// 11.5 us: 5.9 until the last MMA, bound by 11 TB/s of operands from L2 over 128 SMs.
 // Warps per CTA. Alone on its SM a CTA takes 16 (1021 x 2048 x 2048: 11.5 us against 12.4); CTAs of
 // a cluster take 8, and the next launch's clusters find room beside them (128 x 2048 x 2048 on
 // clusters of 8: 8.8 us against 17.1).
@@ -721,8 +731,10 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
 // ----------------------------------------------------------------------------- at most 16 tokens
 // A matrix-vector product reads each weight once: no ring, barrier or tensor memory before the
 // first MMA. A CTA owns RT 16-feature tiles (the SwiGLU: a gate tile and its up tile) over all of
-// K; its 8 warps take the 64-code k-blocks warp, warp + 8, ... and add their int32 sums through
-// shared memory.
+// K; its W warps take the 64-code k-blocks warp, warp + W, ..., D of them in flight, and add their
+// int32 sums through shared memory. Bound by HBM where there are weights enough (1 token, 98304 x
+// 2048: 30.6 us = 6.6 TB/s; 12288 x 2048 SwiGLU 6.0 us = 4.2 TB/s), by the launch's chain of
+// latencies below (2048 x 2048: 2.3 us).
 // Lane (g, t) = (lane / 4, lane % 4) loads codes 16 t .. 16 t + 15 of its k-block of rows g and
 // g + 8 (a quad reads 64 neighbouring bytes), and of tokens g and g + 8. mma.sync m16n8k32 takes 4
 // codes of each row per register: MMA j = 0, 1 is given the words 2 j and 2 j + 1 of both operands,
@@ -994,11 +1006,14 @@ static int launch_i8_reg(const I8Args& a, cudaStream_t st) {
   SDB_CUDA(launch_pdl(gemm_i8_reg_kernel<EP, RT, NT8, W, D, CTAS>, dim3(grid), dim3(32 * W), 0, st, a));
   return B200_OK;
 }
-// Warps per CTA, depth and CTAs per SM, each the best of the shapes measured beside it (us):
-//   SwiGLU, 12288 x 2048: 1 token 6.4 (others 7.7 - 9.9), 16 tokens 8.8 (10.2 - 11.0)
+// Warps per CTA, depth and CTAs per SM, each the best of the shapes measured beside it (us, the
+// others in brackets; all before the finishing operands were read early, which took 0.4 - 0.8 more
+// off each):
+//   SwiGLU, 12288 x 2048: 1 token 6.4 (7.7 - 9.9), 16 tokens 8.8 (10.2 - 11.0)
 //   few tiles (about one CTA per SM), deep K: 16 warps share it (2048 x 6144, 1 token 4.0 against
 //   6.9 on 8 warps); shallow K: 8 warps (2048 x 2048, 13 tokens 3.2 against 3.9 on 16)
-//   many tiles, 8224 x 2048: 1 token 4.8 (6.2 - 8.6), 16 tokens two tiles per CTA 5.8 (6.9 - 9.6)
+//   many tiles, 8224 x 2048: 1 token 4.5 with four CTAs per SM (4.8 - 8.6), 16 tokens two tiles per
+//   CTA 5.8 (6.9 - 9.6)
 template <int EP, int NT8>
 static int dispatch_i8_reg(const I8Args& a, cudaStream_t st) {
   if constexpr (EP == B200_EP_SWIGLU) {
@@ -1063,6 +1078,8 @@ int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k,
     return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: out is not aligned to its elements");
   if (out->lo_format != B200_LO_BF16 && out->lo_format != B200_LO_E4M3)
     return sdb_fail(B200_ERR_ARG, "b200_linear_int8: unknown lo_format");
+  if ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w->row_scale)) & 3)
+    return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: scales are not aligned to their elements");
   I8Args a{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx, 1, 0, 0, 0};
   a.vec = out->ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out->out) & (swiglu ? 7 : 15)) == 0;
   switch (out->epilogue) {

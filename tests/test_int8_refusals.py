@@ -106,7 +106,7 @@ def test_linear_int8(lib, p16):
     for kw in (dict(m=0), dict(m=-1), dict(m=(1 << 30) + 1), dict(n=(1 << 30) + 1), dict(k=0, wk=0), dict(n=0), dict(wk=128), dict(k=40, wk=40),
                dict(k=65552, wk=65552, ldx=65552), dict(ldx=48), dict(ldx=72), dict(q=p16 + 8), dict(data=p16 + 4),
                dict(nv=0), dict(nv=129), dict(ldo=127), dict(out=p16 + 2), dict(ep=2, nv=64), dict(ep=2, ldo=63),
-               dict(ep=2, out=p16 + 1)):
+               dict(ep=2, out=p16 + 1), dict(xs=p16 + 2), dict(rs=p16 + 1)):
         bad(2, **kw)
 
 
