@@ -154,6 +154,8 @@ _lock = threading.Lock()
 def load(path: str | None = None) -> C.CDLL:
     """Load (once) and type the shared library. Raises if it is missing."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -182,7 +184,7 @@ def check(status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(_lib or load(), name)(*args))
+    check(getattr(load(), name)(*args))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

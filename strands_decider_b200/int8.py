@@ -52,19 +52,22 @@ def _place(name: str, t: torch.Tensor) -> tuple[int, int, int]:
     device = t.get_device()
     if device < 0:
         raise ValueError("b200 kernels take CUDA tensors only")
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must be 2-D")
-    rows, k = t.shape
-    return device, rows, k
+    return device, shape[0], shape[1]
 
 
 def _call(device: int, name: str, *args) -> None:
     """One entry point on the device's current stream, with that device current."""
-    if torch.cuda.current_device() == device:
-        _lib.call(name, *args, _lib.raw_stream(device))
+    f = getattr(_lib.load(), name)
+    if torch._C._cuda_getDevice() == device:
+        status = f(*args, _lib.raw_stream(device))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, _lib.raw_stream(device))
+            status = f(*args, _lib.raw_stream(device))
+    if status:
+        _lib.check(status)
 
 
 def _codes_out(out: torch.Tensor | None, scale: torch.Tensor | None, device: int, rows: int, k: int):
