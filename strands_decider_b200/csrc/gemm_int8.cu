@@ -124,6 +124,15 @@ __device__ __forceinline__ void tma_load_5d_pair_hint(void* dst, const CUtensorM
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(0), "r"(v), "l"(policy)
       : "memory");
 }
+// umma_pair_commit for the barrier at this offset in both CTAs of the pair: one instruction of the
+// issuing thread instead of two (8192 x 12288 x 2048 SwiGLU 148.0 -> 144.8 us).
+__device__ __forceinline__ void umma_pair_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"(uint16_t(3))
+      : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -277,7 +286,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
       constexpr uint32_t idesc = umma_idesc_i8(256, 256);
-      const uint32_t empty1 = mapa_shared(smem_addr(empty), 1), acc_full1 = mapa_shared(smem_addr(acc_full), 1);
       int s = 0;
       uint32_t ph = 0, local = 0;
       for (int u = pair; u < n_units; u += n_pairs, ++local) {
@@ -293,12 +301,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 #pragma unroll
           for (int j = 0; j < I8_BK / 32; ++j)  // 32 bytes of K per MMA = +2 in 16-byte units
             umma_pair_i8(acc, ad + 2 * j, bd + 2 * j, idesc, (kt != 0 || j != 0) ? 1u : 0u);
-          umma_pair_commit(smem_addr(&empty[s]));  // both CTAs may refill stage s
-          umma_pair_commit(empty1 + 8u * s);
+          umma_pair_commit_both(&empty[s]);  // both CTAs may refill stage s
           if (++s == SM::STAGES) s = 0, ph ^= 1;
         }
-        umma_pair_commit(smem_addr(&acc_full[ab]));
-        umma_pair_commit(acc_full1 + 8u * ab);
+        umma_pair_commit_both(&acc_full[ab]);
       }
     }
     __syncwarp();
