@@ -509,21 +509,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 // memory ([token][feature], where its operands were), and after one cluster barrier CTA r adds the
 // cluster's sums of tokens r * bt / SPLIT .. and finishes them. No partial sum reaches global
 // memory and none is added atomically.
-//   warp 0  TMA ring; warp 1  MMAs; then all warps drain the accumulator and finish outputs.
-// At these sizes a launch is a chain of latencies. 96 x 8224 x 2048 (clusters of 2), 9.0 us in a row
-// of launches, of which one takes 7.8: 0.5 set-up, 3.7 until the last MMA (8 k-blocks of 28 KB),
-// 0.4 sums to shared memory, 0.7 cluster barrier, 1.3 outputs, 0.8 last barrier. 1021 x 2048 x 2048,
-// 11.5 us: 5.9 until the last MMA, bound by 11 TB/s of operands from L2 over 128 SMs.
-// Warps per CTA. Alone on its SM a CTA takes 16 (1021 x 2048 x 2048: 11.5 us against 12.4); CTAs of
-// a cluster take 8, and the next launch's clusters find room beside them (128 x 2048 x 2048 on
-// clusters of 8: 8.8 us against 17.1).
+//   warp 0  TMA ring; warps 1 and 2  MMAs; then all warps drain the accumulators and finish outputs.
+// Two threads issue MMAs. To issue one costs a thread 35 to 40 ns, more than the tensor cores need for
+// 128 tokens or fewer, so each of two takes every second k-block, with an accumulator of its own (the
+// sums are whole numbers: their order changes nothing). 96 x 8224 x 2048 8.4 us, with one issuer 9.1;
+// 1021 x 2048 x 6144 17.8 : 21.2. (Half of every k-block each: 8.8 and 18.4 us.)
+// At these sizes a launch is a chain of latencies. 96 x 8224 x 2048 (clusters of 2), 8.4 us in a row
+// of launches, of which one takes 7.2: 0.5 set-up, 3 until the last MMA (8 k-blocks of 28 KB),
+// 0.4 sums to shared memory, 0.7 cluster barrier, 1.3 outputs, 0.8 last barrier.
+// Warps per CTA. Alone on its SM a CTA takes 16 (1021 x 2048 x 2048: 10.3 us against 11.3); CTAs of
+// a cluster take 8, and the next launch's clusters find room beside them (32 x 2048 x 6144 on
+// clusters of 8: 7.7 us against 12.6).
 constexpr int i8s_warps(int split) { return split == 1 ? 16 : 8; }
 constexpr int I8S_OP_W = 128 * I8_BK;
 constexpr int I8S_MAX_STAGES = 12;
 constexpr int I8S_RING = 220 * 1024;       // bytes of stages: one CTA per SM
 constexpr int I8S_RING_HALF = 104 * 1024;  // two CTAs per SM
 constexpr int i8s_smem(int stages, int bt) {
-  return 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (2 * I8S_MAX_STAGES + 1) * 8 + 16;
+  return 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (4 * I8S_MAX_STAGES + 1) * 8 + 16;
 }
 
 __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
@@ -547,8 +550,8 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
   uint8_t* sX = sW + stages * I8S_OP_W;
   float* sxs = reinterpret_cast<float*>(sX + stages * x_op);  // [bt] token scales
   uint64_t* full = reinterpret_cast<uint64_t*>(sxs + 128);
-  uint64_t* empty = full + I8S_MAX_STAGES;
-  uint64_t* acc_full = empty + I8S_MAX_STAGES;
+  uint64_t* empty = full + 2 * I8S_MAX_STAGES;
+  uint64_t* acc_full = empty + 2 * I8S_MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   int* sP = reinterpret_cast<int*>(smem);  // [bt][128], once the operands are consumed
 
@@ -556,21 +559,21 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
   const int rank = blockIdx.x % SPLIT, n0 = blockIdx.x / SPLIT * 128, t0 = blockIdx.y * bt;
   const int nk = (a.k + I8_BK - 1) / I8_BK;
   const int kb0 = int(int64_t(rank) * nk / SPLIT), kb1 = int(int64_t(rank + 1) * nk / SPLIT);
-  const uint32_t cols = bt <= 32 ? 32 : bt <= 64 ? 64 : 128;
+  const uint32_t cols = bt <= 32 ? 32 : bt <= 64 ? 64 : 128;  // of one accumulator
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+    for (int b = 0; b < 2 * stages; ++b) {
+      mbar_init(&full[b], 1);
+      mbar_init(&empty[b], 1);
     }
-    mbar_init(acc_full, 1);
+    mbar_init(acc_full, 2);
     mbar_fence_init();
     // weights that lie in HBM start for L2 before the wait for the kernel ahead (a prefetch:
     // nothing is read that it may still write)
     for (int kt = kb0; kt < min(kb1, kb0 + 2 * stages); ++kt) tma_prefetch_2d(&tmW, kt * (I8_BK / 2), n0);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, cols);
+    tmem_alloc(tmem_slot, 2 * cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -583,32 +586,40 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
     sxs[threadIdx.x - 128] = t0 + int(threadIdx.x) - 128 < a.m ? a.xs[t0 + threadIdx.x - 128] : 0.0f;
 
   if (warp == 0) {
+    // k-block i of this CTA lies in stage i % stages; its barriers are number i % (2 stages), so that
+    // a barrier always belongs to the same issuing thread, with an odd number of stages too
     if (lane == 0) {
-      int s = 0;
+      int s = 0, b = 0, be = 0;
       uint32_t ph = 0;
       for (int kt = kb0; kt < kb1; ++kt) {
-        mbar_wait(&empty[s], ph ^ 1, FAULT_GEMM_WAIT_EMPTY);
-        mbar_arrive_expect_tx(&full[s], I8S_OP_W + x_op);
-        tma_load_2d(sW + s * I8S_OP_W, &tmW, &full[s], kt * (I8_BK / 2), n0);
-        tma_load_2d(sX + s * x_op, &tmX, &full[s], kt * (I8_BK / 2), t0);
-        if (++s == stages) s = 0, ph ^= 1;
+        if (kt - kb0 >= stages) {
+          mbar_wait(&empty[be], ph, FAULT_GEMM_WAIT_EMPTY);
+          if (++be == 2 * stages) be = 0, ph ^= 1;
+        }
+        mbar_arrive_expect_tx(&full[b], I8S_OP_W + x_op);
+        tma_load_2d(sW + s * I8S_OP_W, &tmW, &full[b], kt * (I8_BK / 2), n0);
+        tma_load_2d(sX + s * x_op, &tmX, &full[b], kt * (I8_BK / 2), t0);
+        if (++s == stages) s = 0;
+        if (++b == 2 * stages) b = 0;
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_i8(128, bt);
-      int s = 0;
+  } else if (warp <= 2) {
+    if (lane == 0) {  // issuer h: every second k-block, into its own accumulator
+      const uint32_t idesc = umma_idesc_i8(128, bt), h = warp - 1, acc = tmem + h * cols;
+      int b = h;
       uint32_t ph = 0;
-      for (int kt = kb0; kt < kb1; ++kt) {
-        mbar_wait(&full[s], ph, FAULT_GEMM_WAIT_FULL_A);
+      for (int kt = kb0 + h; kt < kb1; kt += 2) {
+        const int s = b >= stages ? b - stages : b;
+        mbar_wait(&full[b], ph, FAULT_GEMM_WAIT_FULL_A);
         tc_fence_after();
         const uint64_t ad = umma_desc_sw128(smem_addr(sW + s * I8S_OP_W));
         const uint64_t bd = umma_desc_sw128(smem_addr(sX + s * x_op));
 #pragma unroll
-        for (int j = 0; j < I8_BK / 32; ++j) umma_i8(tmem, ad + 2 * j, bd + 2 * j, idesc, (kt != kb0 || j != 0) ? 1u : 0u);
-        umma_commit(&empty[s]);
-        if (++s == stages) s = 0, ph ^= 1;
+        for (int j = 0; j < I8_BK / 32; ++j)
+          umma_i8(acc, ad + 2 * j, bd + 2 * j, idesc, (kt >= kb0 + 2 || j != 0) ? 1u : 0u);
+        umma_commit(&empty[b]);
+        if ((b += 2) >= 2 * stages) b -= 2 * stages, ph ^= 1;
       }
       umma_commit(acc_full);
     }
@@ -653,11 +664,13 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
   // ---- sums to shared memory: warp -> lane quarter warp % 4, every second 16 tokens
   const int q = warp & 3;
   for (int c = 16 * (warp >> 2); c < bt; c += 4 * W) {
-    uint32_t v[16];
+    uint32_t v[16], v2[16] = {};
     tmem_ld(tmem + c + (uint32_t(q * 32) << 16), v);
+    if (kb1 - kb0 > 1) tmem_ld(tmem + cols + c + (uint32_t(q * 32) << 16), v2);
     tmem_ld_wait_for(v);
+    tmem_ld_wait_for(v2);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sP[(c + j) * 128 + 32 * q + lane] = int(v[j]);
+    for (int j = 0; j < 16; ++j) sP[(c + j) * 128 + 32 * q + lane] = int(v[j] + v2[j]);
   }
   tc_fence_before();
   if (SPLIT > 1) cluster_sync_all();
@@ -730,7 +743,7 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, cols);
+    tmem_dealloc(tmem, 2 * cols);
   }
 }
 
@@ -988,16 +1001,18 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   const int tiles = n_tiles * m_tiles;
   // K split over a cluster while SMs would idle and every CTA has two k-blocks. Clusters of 8 only
   // for at most 32 tokens: they wait longest for their SMs, and each of their CTAs reads as many sums
-  // as one of 4 (2048 x 6144: 32 tokens 7.8 us against 9.2 on clusters of 4, 128 tokens 16.1 : 10.1).
+  // as one of 4 (2048 x 6144: 32 tokens 7.7 us against 8.3 on clusters of 4, 128 tokens 15.3 : 9.4).
   int split = 1;
   while (split < (a.bt <= 32 ? 8 : 4) && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
-  // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 200 x
-  // 12288 x 2048 22.3 -> 15.5 us), or when that ring holds most of the CTA's K anyway (the next
-  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 13.4 -> 7.3 us); else the deeper
-  // ring (96 x 12288 x 2048: 12.2 us against 13.9).
+  // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 300
+  // x 12288 x 2048 17.8 -> 13.2 us), or when that ring holds most of the CTA's K anyway (the next
+  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 12.1 -> 7.7 us); else the deeper
+  // ring (96 x 12288 x 2048: 8.9 us against 11.7).
   const int stage = I8S_OP_W + a.bt * I8_BK, nkb = (nk + split - 1) / split;
   const bool half = tiles * split > sm_count() || 3 * (I8S_RING_HALF / stage) >= 2 * nkb;
-  a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(2, nkb)});
+  // Two stages at least, for the sums' way through shared memory; three with 256 columns of TMEM, so
+  // that no more CTAs fit on an SM than its TMEM serves.
+  a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(a.bt > 64 ? 3 : 2, nkb)});
   switch (split) {
     case 1: return launch_i8_cluster<EP, LO, 1>(a, n_tiles, m_tiles, st);
     case 2: return launch_i8_cluster<EP, LO, 2>(a, n_tiles, m_tiles, st);

@@ -265,6 +265,30 @@ def test_ragged_token_tiles_come_out_the_same_each_time(m, ep):
         assert ((want.double() - ref).abs() <= 4 * U * ref.abs()).all()
 
 
+@pytest.mark.parametrize("m,n,k,ep", [(200, 12288, 2048, "swiglu"), (32, 2048, 6144, "residual"), (17, 640, 16, "store"),
+                                      (96, 8224, 2048, "store"), (96, 12288, 2048, "swiglu"), (112, 1280, 400, "store"),
+                                      (128, 2048, 16384, "residual"), (250, 2048, 8208, "store")])
+def test_operand_rings_of_every_depth_come_out_the_same_each_time(m, n, k, ep):
+    """Two to twelve stages, odd numbers among them, passed once, in part and many times, by launches
+    that follow one another without a pause; a token alone gives the same bits."""
+    from strands_decider_b200 import int8
+
+    q, s, wq, ws = _operands(m, n, k, 5)
+    q, s, w = q.cuda(), s.cuda() * 0.01, _weight(wq, ws)
+    cols = n // 2 if ep == "swiglu" else n
+    dtype = torch.bfloat16 if ep == "swiglu" else torch.float32
+    base = torch.randn(m, cols, device="cuda").to(dtype)
+    outs = [base.clone() for _ in range(20)]
+    for out in outs:
+        int8.linear(q, s, w, out, epilogue=ep)
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])
+    for i in (0, m // 2, m - 1):
+        one = base[i:i + 1].clone()
+        int8.linear(q[i:i + 1].contiguous(), s[i:i + 1].contiguous(), w, one, epilogue=ep)
+        assert torch.equal(one[0], outs[0][i])
+
+
 @pytest.mark.parametrize("m", [1, 12, 40, 300])
 def test_linear_extreme_codes_at_the_greatest_depth(m):
     """-128 x -128 over k = 65536 is 2^30; signs and single codes come through exactly."""
