@@ -1053,12 +1053,18 @@ template <int EP>
 static int launch_int8(const I8Args& a, cudaStream_t st) {
   if (a.m <= 8) return dispatch_i8_reg<EP, 1>(a, st);
   if (a.m <= I8R_MAX_M) return dispatch_i8_reg<EP, 2>(a, st);
-  // Single CTAs while their 128 x 128 tiles all run at once, two to an SM (300 x 12288 x 2048: 13 us
-  // against 19 on pairs, two rounds of them); pairs beyond (512 x 12288 x 2048: 20 us against 22).
-  // (Pairs with tiles of 128 tokens, to even out their rounds, were slower: 0.8 of the time of 256.)
+  // Single CTAs while each 128 x 128 tile has an SM (1021 x 2048 x 6144: 17.8 us, pairs 25). With two
+  // of them to an SM, pairs if one round of them does (2000 x 2048 x 6144: 27.2 us against 46.2; 300 x
+  // 8224 x 2048: 12.5 : 13.1), unless K is short, where two CTAs hide each other's set-up and outputs
+  // (200 x 16384 x 512: 9.2 : 7.5; at K = 1024 both are within 8 %). Where pairs would take two
+  // rounds, single CTAs (300 x 12288 x 2048: 13.0 us against 17.7). Pairs beyond (512 x 12288 x 2048:
+  // 20 us against 22). Tiles of 128 tokens, to even out the pairs' rounds, take 0.8 of the time of
+  // tiles of 256 for half the work: the issue of an MMA takes as long.
+  const int sms = sm_count();
   const int64_t tiles = int64_t((a.o.n_valid + 127) / 128) * ((a.m + 127) / 128);
+  const int64_t pair_tiles = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
   constexpr bool SW = EP == B200_EP_SWIGLU;
-  if (tiles <= 2 * sm_count()) {
+  if (tiles <= sms || (tiles <= 2 * sms && (2 * pair_tiles > sms || a.k <= 1024))) {
     if constexpr (SW) {
       if (a.o.lo_offset) return launch_i8_split<EP, true>(a, st);
     }

@@ -186,7 +186,7 @@ def _ref(q, s, wq, ws):
 SHAPES = [(1, 1, 16), (1, 130, 64), (2, 2048, 2048), (7, 1000, 144), (8, 96, 8208), (9, 257, 1040), (16, 2304, 512),
           (17, 640, 2048), (31, 33, 48), (33, 129, 6144), (64, 1153, 528), (65, 256, 4112), (96, 8224, 256),
           (127, 384, 1024), (129, 127, 272), (200, 2048, 2032), (255, 600, 2064), (257, 520, 128), (511, 1025, 400),
-          (1021, 2048, 2048), (2050, 4200, 336), (2050, 4201, 144),
+          (1021, 2048, 2048), (1290, 2040, 1040), (2050, 4200, 336), (2050, 4201, 144),
           (4099, 2600, 1040), (9001, 1290, 144)]
 
 
@@ -207,7 +207,7 @@ def test_linear_store_and_residual(m, n, k):
 
 
 SWIGLU_SHAPES = [(1, 128, 16), (1, 12288, 256), (5, 256, 144), (13, 1152, 2048), (16, 128, 1040), (24, 640, 528),
-                 (96, 1024, 2048), (130, 384, 400), (300, 2432, 1024), (1030, 1280, 272), (2050, 4224, 160),
+                 (96, 1024, 2048), (130, 384, 400), (300, 2432, 1024), (600, 5504, 1040), (1030, 1280, 272), (2050, 4224, 160),
                  (3333, 3200, 144)]
 
 
