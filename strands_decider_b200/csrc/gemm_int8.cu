@@ -7,7 +7,7 @@
 // scales are applied in one order (i8_value), so a row's result is the same bits in every kernel,
 // batch and split.
 //
-//   gemm_i8_pair_kernel   CTA pairs, 256 features x 256 tokens, persistent (large products)
+//   gemm_i8_pair_kernel   CTA pairs, 256 features x 256 or 192 tokens, persistent (large products)
 //   gemm_i8_split_kernel  one CTA per 128 features x up to 128 tokens and K range; the K ranges of
 //                         a tile are a cluster that adds its sums through distributed shared memory
 //   gemm_i8_reg_kernel    at most 16 tokens: weights through registers into mma.sync
@@ -26,7 +26,8 @@ struct I8Args {
   b200_linear_out o;
   int m, n, k, ldx;
   int ngroup;           // pair kernel: feature tiles per group
-  int bt, stages;       // split kernel: tokens per tile, ring depth
+  int bt;               // pair and split kernel: tokens per tile
+  int stages;           // split kernel: ring depth
   int vec;              // split kernel: every fourth output of a row is aligned to four outputs
 };
 
@@ -148,12 +149,12 @@ __device__ __forceinline__ void tma_store_wait_read() {
 __device__ __forceinline__ void tma_store_wait_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ----------------------------------------------------------------------------- CTA pairs
-// Tile: 256 features (128 per CTA) x 256 tokens, K in stages of 128 codes (four MMAs of K = 32).
+// Tile: 256 features (128 per CTA) x bt tokens (256, or 192), K in stages of 128 codes (four MMAs of K = 32).
 // Each CTA loads its 128 weight rows and its half of the tokens; the pair's MMA reads both halves.
 //   warp 0      TMA ring (both CTAs; bytes signalled on the leader's full barrier)
 //   warp 1      the leader's lane 0 issues the MMAs into one of two 256-column accumulators
 //   warps 2..9  epilogue: TMEM lane quarter warp % 4, token half (warp - 2) / 4
-//               (128 tokens, 16 or 32 at a time; the next ones leave TMEM while these are finished)
+//               (bt / 2 tokens, 16 or 32 at a time; the next ones leave TMEM while these are finished)
 // 256 x 256 is the largest tile that leaves room for a second accumulator, which the next tile's
 // products need while this one is finished: the main loop alone runs at 3425-3496 Tops/s (8192 and
 // 18944 x 12288 x 2048), and with it 13 TB/s of operands cross from L2. What is lost on top is
@@ -222,7 +223,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   const uint32_t rank = cluster_ctarank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nk = (a.k + I8_BK - 1) / I8_BK;
-  const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + 255) / 256;
+  const int bt = a.bt, th = bt / 2;
+  const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + bt - 1) / bt;
   const int n_units = n_tiles * m_tiles;
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   // groups of ngroup feature tiles; token tiles within a group, so that the weights a group
@@ -269,11 +271,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       for (int u = pair; u < n_units; u += n_pairs) {
         int mt, nt;
         tile_of(u, mt, nt);
-        const int n0 = nt * 256 + int(rank) * 128, t0 = mt * 256 + int(rank) * 128;
+        const int n0 = nt * 256 + int(rank) * 128, t0 = mt * bt + int(rank) * th;
         for (int kt = 0; kt < nk; ++kt) {
           mbar_wait(&empty[s], ph ^ 1, FAULT_GEMM_WAIT_EMPTY);
           const uint32_t fb = full0 + 8u * s;
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * SM::STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (SM::OP + th * I8_BK));
           if constexpr (EP == B200_EP_SWIGLU)
             tma_load_5d_pair_hint(sW + s * SM::OP, &tmW, fb, kt * (I8_BK / 2), n0 / 128, keep);
           else
@@ -285,7 +287,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_i8(256, 256);
+      const uint32_t idesc = umma_idesc_i8(256, bt);
       int s = 0;
       uint32_t ph = 0, local = 0;
       for (int u = pair; u < n_units; u += n_pairs, ++local) {
@@ -335,7 +337,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     auto scales = [&](int u) {
       int mt, nt;
       tile_of(u, mt, nt);
-      const int n = nt * 256 + int(rank) * 128 + row, t0 = mt * 256 + 128 * hf;
+      const int n = nt * 256 + int(rank) * 128 + row, t0 = mt * bt + th * hf;
       ws_next = n < a.n ? a.ws[n] : 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) xs_next[i] = t0 + 32 * i + lane < a.m ? a.xs[t0 + 32 * i + lane] : 0.0f;
@@ -352,8 +354,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       for (; pu < n_units; pu += n_pairs, pc = 0) {
         int mt, nt;
         tile_of(pu, mt, nt);
-        n0 = nt * 256 + int(rank) * 128, t0 = mt * 256 + 128 * hf;
-        if (pc < chunks(n0, a.m - t0)) break;
+        n0 = nt * 256 + int(rank) * 128, t0 = mt * bt + th * hf;
+        if (pc < chunks(n0, min(th, a.m - t0))) break;
       }
       if (pu >= n_units) return;
       if (lane == 0) {
@@ -374,9 +376,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       int mt, nt;
       tile_of(u, mt, nt);
       const int n0 = nt * 256 + int(rank) * 128, n = n0 + row;
-      const int t0 = mt * 256 + 128 * hf, left = a.m - t0;  // this warp's first token, tokens from it on
+      const int t0 = mt * bt + th * hf, left = min(th, a.m - t0);  // this warp's first token, and how many
       const uint32_t ab = local & 1, aph = (local >> 1) & 1;
-      const uint32_t tl = tmem + ab * 256 + 128 * hf + (uint32_t(q * 32) << 16);
+      const uint32_t tl = tmem + ab * 256 + th * hf + (uint32_t(q * 32) << 16);
       const float ws = ws_next;
       __syncwarp();
 #pragma unroll
@@ -942,17 +944,26 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   if (r != B200_OK) return r;
   int dev = 0;
   SDB_CUDA(cudaGetDevice(&dev));
+  // Tiles of 192 tokens where the pairs need no more rounds of them: a k-block takes 0.32 us instead of
+  // 0.34 and the outputs less (1536 x 2048 x 2048 15.7 -> 14.3 us, 2560 x 2048 x 6144 43.9 -> 41.8); with
+  // another round they lose (4096 x 2048 x 2048: 29.2 us against 25.6).
+  const int n_tiles = (a.o.n_valid + 255) / 256;
+  auto rounds = [&](int bt) {
+    const int64_t units = int64_t(n_tiles) * ((a.m + bt - 1) / bt);
+    return (units + max_pairs_dev[dev] - 1) / max_pairs_dev[dev];
+  };
+  a.bt = rounds(192) == rounds(256) ? 192 : 256;
   CUtensorMap mw, mx, mo;
   constexpr bool SW = EP == B200_EP_SWIGLU;
   if (int rc = SW ? i8_swiglu_map(&mw, a.w, a.o.n_valid / 128, a.k) : i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
-  if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, 128)) return rc;
+  if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, a.bt / 2)) return rc;
   mo = mw;  // not read
   if constexpr (OUT == I8_TMA) {
     if (int rc = encode_store_tile(&mo, a.o.out, SW ? 2 : 4, a.m, SW ? a.o.n_valid / 2 : a.o.n_valid, a.o.ldo, SW ? 32 : 16,
                                    SW ? 16 : 32))
       return rc;
   }
-  const int n_tiles = (a.o.n_valid + 255) / 256, m_tiles = (a.m + 255) / 256;
+  const int m_tiles = (a.m + a.bt - 1) / a.bt;
   // weights beyond what L2 keeps beside the activation stream: groups of about 40 MB
   const double tile_bytes = 256.0 * a.k;
   const int groups = n_tiles * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles * tile_bytes / 40e6));
@@ -1055,11 +1066,10 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   if (a.m <= I8R_MAX_M) return dispatch_i8_reg<EP, 2>(a, st);
   // Single CTAs while each 128 x 128 tile has an SM (1021 x 2048 x 6144: 17.8 us, pairs 25). With two
   // of them to an SM, pairs if one round of them does (2000 x 2048 x 6144: 27.2 us against 46.2; 300 x
-  // 8224 x 2048: 12.5 : 13.1), unless K is short, where two CTAs hide each other's set-up and outputs
+  // 8224 x 2048: 11.7 : 13.1), unless K is short, where two CTAs hide each other's set-up and outputs
   // (200 x 16384 x 512: 9.2 : 7.5; at K = 1024 both are within 8 %). Where pairs would take two
   // rounds, single CTAs (300 x 12288 x 2048: 13.0 us against 17.7). Pairs beyond (512 x 12288 x 2048:
-  // 20 us against 22). Tiles of 128 tokens, to even out the pairs' rounds, take 0.8 of the time of
-  // tiles of 256 for half the work: the issue of an MMA takes as long.
+  // 18.6 us against 22).
   const int sms = sm_count();
   const int64_t tiles = int64_t((a.o.n_valid + 127) / 128) * ((a.m + 127) / 128);
   const int64_t pair_tiles = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);

@@ -207,7 +207,7 @@ def test_linear_store_and_residual(m, n, k):
 
 
 SWIGLU_SHAPES = [(1, 128, 16), (1, 12288, 256), (5, 256, 144), (13, 1152, 2048), (16, 128, 1040), (24, 640, 528),
-                 (96, 1024, 2048), (130, 384, 400), (300, 2432, 1024), (600, 5504, 1040), (1030, 1280, 272), (2050, 4224, 160),
+                 (96, 1024, 2048), (130, 384, 400), (300, 2432, 1024), (600, 5504, 1040), (500, 5504, 1040), (1030, 1280, 272), (2050, 4224, 160),
                  (3333, 3200, 144)]
 
 
