@@ -513,12 +513,10 @@ constexpr int kMaxDevices = 64;
 // read as zero. Defined in gemm.cu.
 int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
                       const uint32_t* box);
-// A row-major [rows, cols] output of bf16 or fp32 (elem_bytes 2 or 4; ld elements per row) for
-// tiled loads and stores of box_cols x box_rows from unswizzled shared memory. Rows past the end are
-// not touched; columns are cut at whole 16 bytes, so cols * elem_bytes must be a multiple of 16.
-// Defined in gemm.cu.
-int encode_store_tile(CUtensorMap* map, const void* base, int elem_bytes, int rows, int cols, int64_t ld,
-                      int box_rows, int box_cols);
+// A row-major [rows, cols] bf16 output (ld elements per row) for tiled stores of box_cols x box_rows
+// from unswizzled shared memory. Rows past the end are not touched; columns are cut at whole 16
+// bytes, so cols must be a multiple of 8. Defined in gemm.cu.
+int encode_store_tile(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows, int box_cols);
 
 // Kernel attributes (such as the dynamic shared-memory limit) are per device, and one process
 // may drive several GPUs from several host threads. A DeviceOnce runs a set-up step once per

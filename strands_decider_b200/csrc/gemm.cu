@@ -1074,17 +1074,15 @@ int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64
   return B200_OK;
 }
 
-int encode_store_tile(CUtensorMap* map, const void* base, int elem_bytes, int rows, int cols, int64_t ld,
-                      int box_rows, int box_cols) {
+int encode_store_tile(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows, int box_cols) {
   if (int rc = get_encode_fn()) return rc;
-  if (int64_t(cols) * elem_bytes % 16 != 0) return sdb_fail(B200_ERR_SHAPE, "encode_store_tile: cols end inside 16 bytes");
+  if (cols % 8 != 0) return sdb_fail(B200_ERR_SHAPE, "encode_store_tile: cols end inside 16 bytes");
   const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
-  const cuuint64_t strides[1] = {cuuint64_t(ld) * elem_bytes};
+  const cuuint64_t strides[1] = {cuuint64_t(ld) * 2};
   const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = g_encode(map, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                              2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return sdb_fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed for an output tile");
   return B200_OK;

@@ -158,28 +158,28 @@ __device__ __forceinline__ void tma_store_wait_done() { asm volatile("cp.async.b
 // 256 x 256 is the largest tile that leaves room for a second accumulator, which the next tile's
 // products need while this one is finished: the main loop alone runs at 3425-3496 Tops/s (8192 and
 // 18944 x 12288 x 2048), and with it 13 TB/s of operands cross from L2. What is lost on top is
-// the epilogue's instructions and bytes: 8192 x 12288 x 2048 SwiGLU 148 us = 2.78 Pops/s, 65536
-// tokens 1149 us; in a seconds-long run the 1000 W cap sets 1.47 GHz and 1325 us = 2.49 Pops/s.
-// 65536 x 2048 x 6144 with the residual: 602 us = 2.74 Pops/s; x 2048: 289 us = 4.2 TB/s.
+// the epilogue's instructions and bytes: 8192 x 12288 x 2048 SwiGLU 143 us = 2.88 Pops/s, 65536
+// tokens 1130 us; in a seconds-long run the 1000 W cap sets 1.47 GHz and 1325 us = 2.49 Pops/s.
+// 65536 x 2048 x 6144 with the residual: 567 us = 2.91 Pops/s; x 2048: 262 us = 4.6 TB/s.
 constexpr int I8P_THREADS = 320;
 constexpr int I8P_EPI_WARPS = 8;
-// How the pair kernel writes: from registers (any alignment), the SwiGLU with a low plane, or 32
-// features x 16 tokens (the SwiGLU: 16 x 32) at a time from shared memory by TMA (16-byte aligned
-// rows: stores of 4 or 2 bytes and their addresses were the longest part of the epilogue). With a
-// residual the tile is loaded by TMA two tiles ahead, added to where it lies, and stored.
-enum I8Out { I8_DIRECT = 0, I8_PLANES = 1, I8_TMA = 2 };
+// How the pair kernel writes: from registers (the fp32 store, where 32 lanes write 128 bytes of a row;
+// any alignment), the SwiGLU with a low plane, or through shared memory (rows aligned to 16 bytes).
+// The SwiGLU's 32 tokens x 16 features go out by TMA: stores of 2 bytes and their addresses were the
+// longest part of its epilogue. A residual's 16 tokens x 32 features are turned, so that it is read
+// and written 16 bytes a lane (65536 x 2048 x 2048 262 us, from registers 320; by TMA 289, its small
+// copies queued with the operands').
+enum I8Out { I8_DIRECT = 0, I8_PLANES = 1, I8_STAGED = 2 };
 
 template <int EP, int OUT>
 struct I8PairSmem {
   static constexpr int OP = 128 * I8_BK;                    // one operand of a stage
   static constexpr int STAGE = 2 * OP;
-  // the fp32 tiles of TMA stores take a stage's room, those of a residual two
-  static constexpr int STAGES = OUT != I8_TMA || EP == B200_EP_SWIGLU ? 6 : EP == B200_EP_STORE ? 5 : 4;
-  static constexpr int OT = OUT == I8_TMA ? 16 * 32 * (EP == B200_EP_SWIGLU ? 2 : 4) : 0;  // one tile of a store
-  static constexpr int OTS = EP == B200_EP_RESID_ADD ? 4 : 2;                              // tiles per epilogue warp
+  static constexpr int STAGES = 6;
+  static constexpr int TILES = OUT == I8_STAGED ? 2048 : 0;  // each epilogue warp's: one in fp32 or two in bf16
   static constexpr int XS = I8P_EPI_WARPS * 128 * 4;        // each epilogue warp's token scales
-  static constexpr int BARS = 2 * STAGES + 4 + 4 * I8P_EPI_WARPS;
-  static constexpr int TOTAL = 1024 + STAGES * STAGE + OTS * I8P_EPI_WARPS * OT + XS + BARS * 8 + 16;
+  static constexpr int BARS = 2 * STAGES + 4;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE + I8P_EPI_WARPS * TILES + XS + BARS * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -210,14 +210,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = sW + SM::STAGES * SM::OP;
-  uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp][OTS] tiles of TMA stores
-  float* sxs = reinterpret_cast<float*>(sO + SM::OTS * I8P_EPI_WARPS * SM::OT);
+  uint8_t* sO = sX + SM::STAGES * SM::OP;  // [epilogue warp] tiles
+  float* sxs = reinterpret_cast<float*>(sO + I8P_EPI_WARPS * SM::TILES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sxs + SM::XS / 4);
   uint64_t* full = bars;                            // the leader's are used
   uint64_t* empty = bars + SM::STAGES;              // both CTAs'
   uint64_t* acc_full = bars + 2 * SM::STAGES;       // [2], both CTAs'
   uint64_t* acc_empty = bars + 2 * SM::STAGES + 2;  // [2], the leader's are used
-  uint64_t* res_full = bars + 2 * SM::STAGES + 4;   // [epilogue warp][4]: a residual tile has landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SM::BARS);
 
   const uint32_t rank = cluster_ctarank();
@@ -246,7 +245,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2 * I8P_EPI_WARPS);
     }
-    for (int b = 0; b < 4 * I8P_EPI_WARPS; ++b) mbar_init(&res_full[b], 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -314,14 +312,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     const int q = warp & 3, hf = (warp - 2) >> 2;
     const uint32_t acc_empty0 = mapa_shared(smem_addr(acc_empty), 0);
     float* xs = sxs + (warp - 2) * 128;  // scales of this warp's 128 tokens
-    uint8_t* tiles = sO + SM::OTS * (warp - 2) * SM::OT;
+    uint8_t* tiles = sO + (warp - 2) * SM::TILES;
     // Store tiles: the g-th tile that this warp stores (tiles with nothing to store are left out, and
     // not written either) lies in buffer g % 2, free once the store before the last has read it.
     uint32_t sg = 0;
     auto free_tile = [&]() {
       if (lane == 0) tma_store_wait_read<1>();
       __syncwarp();
-      return tiles + (sg++ & 1) * SM::OT;
+      return tiles + (sg++ & 1) * 1024;
     };
     auto tile_store = [&](const void* tile, int x, int y) {
       fence_proxy_async_smem();
@@ -343,34 +341,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
       for (int i = 0; i < 4; ++i) xs_next[i] = t0 + 32 * i + lane < a.m ? a.xs[t0 + 32 * i + lane] : 0.0f;
     };
     if (pair < n_units) scales(pair);
-    // Residual tiles: the g-th tile of this warp (over its units, empty ones left out) goes through
-    // buffer g % 4. A tile is asked for two tiles ahead, when the store of the tile that was in its
-    // buffer is the last but one.
-    int pu = pair, pc = 0;          // the next tile to ask for: unit, 16-token chunk
-    uint32_t pg = 0, rg = 0;        // tiles asked for, tiles finished
-    auto chunks = [&](int n0, int left) { return n0 + 32 * q < a.o.n_valid ? min(8, max(0, left + 15) / 16) : 0; };
-    auto ask = [&]() {
-      int n0 = 0, t0 = 0;
-      for (; pu < n_units; pu += n_pairs, pc = 0) {
-        int mt, nt;
-        tile_of(pu, mt, nt);
-        n0 = nt * 256 + int(rank) * 128, t0 = mt * bt + th * hf;
-        if (pc < chunks(n0, min(th, a.m - t0))) break;
-      }
-      if (pu >= n_units) return;
-      if (lane == 0) {
-        uint64_t* bar = &res_full[4 * (warp - 2) + (pg & 3)];
-        tma_store_wait_read<1>();
-        mbar_arrive_expect_tx(bar, SM::OT);
-        tma_load_2d(tiles + (pg & 3) * SM::OT, &tmO, bar, n0 + 32 * q, t0 + 16 * pc);
-      }
-      ++pc;
-      ++pg;
+    // Sums that a residual is added to go through a [16 tokens][32 features] tile, after which this
+    // lane has four features, lf .. lf + 3, of every fourth token from lr on. Their residuals are read
+    // three chunks of 16 tokens ahead, over the end of a unit too (two ahead: 1200 x 2048 x 2048 13.1 us
+    // against 12.2).
+    constexpr bool RES = OUT == I8_STAGED && EP == B200_EP_RESID_ADD;
+    const int lr = lane >> 3, lf = 4 * (lane & 7);
+    auto out_at = [&](int u, int& left) {
+      int mt, nt;
+      tile_of(u, mt, nt);
+      const int t0 = mt * bt + th * hf, f = nt * 256 + int(rank) * 128 + 32 * q + lf;
+      left = f < a.o.n_valid ? min(th, a.m - t0) - lr : 0;
+      return static_cast<float*>(a.o.out) + size_t(t0 + lr) * a.o.ldo + f;
     };
-    if constexpr (EP == B200_EP_RESID_ADD && OUT == I8_TMA) {
-      ask();
-      ask();
+    float4 res[4][4];
+    auto residuals = [&](int c, float* p, int left) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * c + 4 * i < left) res[c & 3][i] = *reinterpret_cast<const float4*>(p + size_t(16 * c + 4 * i) * a.o.ldo);
+    };
+    float* pn = nullptr;
+    int ln = 0;
+    if constexpr (RES) {
+      if (pair < n_units) {
+        pn = out_at(pair, ln);
+        residuals(0, pn, ln);
+        residuals(1, pn, ln);
+        residuals(2, pn, ln);
+      }
     }
+    // The warp has an accumulator's sums in registers: the next products may overwrite it. Relaxed: no
+    // memory is handed over, and a release would wait for this warp's stores.
+    auto acc_read = [&](uint32_t ab) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty0 + 8u * ab) : "memory");
+    };
     uint32_t local = 0;
     for (int u = pair; u < n_units; u += n_pairs, ++local) {
       int mt, nt;
@@ -398,11 +405,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
         for (int c = 0; c < 4; ++c) {
           tmem_ld_wait_for(v[c & 1]);
           if (c < 3) tmem_ld(tl + 32 * (c + 1), v[(c + 1) & 1]);
+          else acc_read(ab);
           const int l = left - 32 * c;
           const size_t idx = idx0 + size_t(32 * c) * a.o.ldo;
           if (!valid || l <= 0) continue;  // the whole warp
           uint8_t* tile = nullptr;
-          if constexpr (OUT == I8_TMA) tile = free_tile();
+          if constexpr (OUT == I8_STAGED) tile = free_tile();
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 x = *reinterpret_cast<const float4*>(xs + 32 * c + j);
@@ -413,19 +421,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
               const float y1 = i8_value(int(v[c & 1][j + e + 1]), xe[e + 1], ws);
               const float other = __shfl_xor_sync(0xffffffffu, up ? y0 : y1, 16);
               const float g = up ? other : y0, uv = up ? y1 : other;
-              if constexpr (OUT == I8_TMA)
+              if constexpr (OUT == I8_STAGED)
                 reinterpret_cast<uint16_t*>(tile)[16 * (j + e) + lane] = f32_to_bf16_rn(swiglu(g, uv));
               else if (j + e + (up ? 1 : 0) < l)
                 store_swiglu<OUT == I8_PLANES>(a.o, idx + size_t(j + e) * a.o.ldo, g, uv);
             }
           }
-          if constexpr (OUT == I8_TMA) tile_store(tile, n0 / 2 + 16 * q, t0 + 32 * c);
+          if constexpr (OUT == I8_STAGED) tile_store(tile, n0 / 2 + 16 * q, t0 + 32 * c);
         }
       } else {
         float* p = static_cast<float*>(a.o.out) + size_t(t0) * a.o.ldo + n;
         const bool valid = n < a.o.n_valid;
+        float* const po = pn;
+        const int lo = ln;
+        if constexpr (RES) {
+          ln = 0;
+          if (u + n_pairs < n_units) pn = out_at(u + n_pairs, ln);
+        }
         // columns in hand (and as many ahead)
-        constexpr int CW = EP == B200_EP_RESID_ADD || OUT == I8_TMA ? 16 : 32;
+        constexpr int CW = EP == B200_EP_RESID_ADD ? 16 : 32;
         float r[2][CW];
         auto residual = [&](int c) {  // chunk c's residual, read while the chunk before is finished
           if constexpr (EP == B200_EP_RESID_ADD && OUT == I8_DIRECT) {
@@ -445,31 +459,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
           if (c + 1 < 128 / CW) {
             tmem_ld(tl + CW * (c + 1), v[(c + 1) & 1]);
             residual(c + 1);
+          } else {
+            acc_read(ab);
           }
           const int l = left - CW * c;
-          if constexpr (OUT == I8_TMA && EP == B200_EP_RESID_ADD) {
-            if (c < chunks(n0, left)) {
-              ask();
-              mbar_wait(&res_full[4 * (warp - 2) + (rg & 3)], (rg >> 2) & 1, FAULT_GEMM_WAIT_FULL_W);
-              __syncwarp();
-              float* tile = reinterpret_cast<float*>(tiles + (rg & 3) * SM::OT) + lane;
-#pragma unroll
-              for (int j = 0; j < CW; j += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(xs + CW * c + j);
-                const float xe[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float* t = tile + 32 * (j + e);
-                  *t = __fadd_rn(*t, i8_value(int(v[c & 1][j + e]), xe[e], ws));
-                }
-              }
-              tile_store(tiles + (rg & 3) * SM::OT, n0 + 32 * q, t0 + CW * c);
-              ++rg;
-            }
-          } else if constexpr (OUT == I8_TMA) {
-            if (c < chunks(n0, left)) {
-              uint8_t* const dst = free_tile();
-              float* tile = reinterpret_cast<float*>(dst) + lane;
+          if constexpr (RES) {
+            if (c < 5) residuals(c + 3, po, lo);
+            else residuals(c - 5, pn, ln);
+            if (l > 0) {  // the whole warp
+              float* const dst = reinterpret_cast<float*>(tiles);
+              float* tile = dst + lane;
 #pragma unroll
               for (int j = 0; j < CW; j += 4) {
                 const float4 x = *reinterpret_cast<const float4*>(xs + CW * c + j);
@@ -478,7 +477,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
                 tile[32 * (j + 2)] = i8_value(int(v[c & 1][j + 2]), x.z, ws);
                 tile[32 * (j + 3)] = i8_value(int(v[c & 1][j + 3]), x.w, ws);
               }
-              tile_store(dst, n0 + 32 * q, t0 + CW * c);
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float4 y = *reinterpret_cast<const float4*>(dst + 32 * (4 * i + lr) + lf);
+                const float4 r4 = res[c & 3][i];
+                y = make_float4(__fadd_rn(r4.x, y.x), __fadd_rn(r4.y, y.y), __fadd_rn(r4.z, y.z), __fadd_rn(r4.w, y.w));
+                if (16 * c + 4 * i < lo) *reinterpret_cast<float4*>(po + size_t(16 * c + 4 * i) * a.o.ldo) = y;
+              }
             }
           } else if (valid) {
             float* pc = p + size_t(CW * c) * a.o.ldo;
@@ -488,13 +494,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
           __syncwarp();
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * ab);
     }
   }
 
-  if constexpr (OUT == I8_TMA) {
+  if constexpr (OUT == I8_STAGED && EP == B200_EP_SWIGLU) {
     if (warp >= 2 && lane == 0) tma_store_wait_done();
   }
   tc_fence_before();
@@ -958,10 +961,8 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   if (int rc = SW ? i8_swiglu_map(&mw, a.w, a.o.n_valid / 128, a.k) : i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
   if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, a.bt / 2)) return rc;
   mo = mw;  // not read
-  if constexpr (OUT == I8_TMA) {
-    if (int rc = encode_store_tile(&mo, a.o.out, SW ? 2 : 4, a.m, SW ? a.o.n_valid / 2 : a.o.n_valid, a.o.ldo, SW ? 32 : 16,
-                                   SW ? 16 : 32))
-      return rc;
+  if constexpr (SW && OUT == I8_STAGED) {
+    if (int rc = encode_store_tile(&mo, a.o.out, a.m, a.o.n_valid / 2, a.o.ldo, 32, 16)) return rc;
   }
   const int m_tiles = (a.m + a.bt - 1) / a.bt;
   // weights beyond what L2 keeps beside the activation stream: groups of about 40 MB
@@ -1083,10 +1084,11 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   if constexpr (SW) {
     if (a.o.lo_offset) return launch_i8_pair<EP, I8_PLANES>(a, st);
   }
-  // A TMA tile ends at a whole 16 bytes: with 3999 outputs it would write the 4000th column too.
-  if (int64_t(a.o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o.out) & 15) == 0 &&
-      (SW || a.o.n_valid % 4 == 0))
-    return launch_i8_pair<EP, I8_TMA>(a, st);
+  if constexpr (EP != B200_EP_STORE) {
+    if (int64_t(a.o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o.out) & 15) == 0 &&
+        (SW || a.o.n_valid % 4 == 0))
+      return launch_i8_pair<EP, I8_STAGED>(a, st);
+  }
   return launch_i8_pair<EP, I8_DIRECT>(a, st);
 }
 
