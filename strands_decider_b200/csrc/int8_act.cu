@@ -11,7 +11,7 @@
 // Every row is read once: its elements stay in the registers of the threads that share it while
 // the sum, the maximum and the codes follow one another. Bound by HBM where there are rows enough:
 // norm 65536 x 2048 115 us = 5.8 TB/s (then by issue: about 25 instructions an element), 12288 x 2048
-// with an fp32 delta 50.7 us = 6.5 TB/s; codes of 65536 x 6144 bf16 210 us = 5.8 TB/s, of 12288 x
+// with an fp32 delta 50.7 us = 6.5 TB/s; codes of 65536 x 6144 bf16 173 us = 7.0 TB/s, of 12288 x
 // 2048 two planes 19.6 us = 5.7 TB/s; one row of 2048 is a chain of latencies, 2.2 and 1.6 us.
 #include "common.cuh"
 
@@ -161,16 +161,32 @@ __global__ void __launch_bounds__(row_threads<TPR>()) rmsnorm_int8_kernel(const 
   const double ss = row_sum<TPR>((s0 + s1) + (s2 + s3), psum);
   const float r = float(rsqrt(ss / double(a.k) + double(a.eps)));
   uint32_t mx = 0u;
+  auto scaled = [&](float4& u, const float4& w) {
+    u.x = __fmul_rn(__fmul_rn(u.x, r), 1.0f + w.x);
+    u.y = __fmul_rn(__fmul_rn(u.y, r), 1.0f + w.y);
+    u.z = __fmul_rn(__fmul_rn(u.z, r), 1.0f + w.z);
+    u.w = __fmul_rn(__fmul_rn(u.w, r), 1.0f + w.w);
+    mx = max(max(max(mx, abs_bits(u.x)), abs_bits(u.y)), max(abs_bits(u.z), abs_bits(u.w)));
+  };
+  const float4* wr = reinterpret_cast<const float4*>(a.w);
+  // A warp's weights in batches, whose loads are in flight together (3844 x 784 9.0 -> 6.4 us, 20000 x
+  // 1392 39.7 -> 32.6). Not of its longest rows, whose registers they would take (65536 x 2048: 202 us
+  // against 116), and not in blocks of a row, of which enough are resident (28162 x 2512 73 : 68).
+  constexpr int B = TPR > 32 || NV > 12 ? 1 : NV % 4 == 0 ? 4 : NV % 3 == 0 ? 3 : NV;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int j = t + TPR * i;
-    if (j < n4) {
-      const float4 w = __ldg(reinterpret_cast<const float4*>(a.w) + j);
-      v[i].x = __fmul_rn(__fmul_rn(v[i].x, r), 1.0f + w.x);
-      v[i].y = __fmul_rn(__fmul_rn(v[i].y, r), 1.0f + w.y);
-      v[i].z = __fmul_rn(__fmul_rn(v[i].z, r), 1.0f + w.z);
-      v[i].w = __fmul_rn(__fmul_rn(v[i].w, r), 1.0f + w.w);
-      mx = max(max(max(mx, abs_bits(v[i].x)), abs_bits(v[i].y)), max(abs_bits(v[i].z), abs_bits(v[i].w)));
+  for (int i0 = 0; i0 < NV; i0 += B) {
+    if constexpr (B == 1) {
+      const int j = t + TPR * i0;
+      if (j < n4) scaled(v[i0], __ldg(wr + j));
+    } else {
+      float4 w[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int j = t + TPR * (i0 + i);
+        w[i] = j < n4 ? __ldg(wr + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) scaled(v[i0 + i], w[i]);  // past the row's end: zeros
     }
   }
   mx = row_max<TPR>(mx, pmax);
@@ -258,7 +274,9 @@ __global__ void __launch_bounds__(row_threads<TPR>()) quantize_int8_kernel(const
 // x 2048: 19.5 us with 128 threads a row, 22.1 with 32; an fp32 delta at 12288 x 2048: 50.6 against
 // 59.2; no delta at 65536 x 2048: 116 us with 32, 123 with 128). Four times as many while the
 // device has under 512 threads per SM and the row has work for them (1 x 2048: 2.1 us against 2.5).
-// Rows of at most 32 groups take 8 lanes, four rows to a warp.
+// Rows of at most 32 groups take 8 lanes, four rows to a warp. A thread's groups are 1, 2, 3, 4, 6, 8,
+// 12 or 16: registers for twice as many as the row has would leave fewer rows in flight (codes of
+// 65536 x 6144 bf16 in 8 groups 209 us, in 6 174; of 12072 x 2400 30.6 : 18.8).
 struct RowShape {
   int tpr, nv;
 };
@@ -267,7 +285,7 @@ static RowShape row_shape(int rows, int units, int cap) {
   while (tpr < 512 && (units > cap * tpr || (int64_t(rows) * tpr < 512 * int64_t(sm_count()) && units > tpr))) tpr *= 4;
   if (units > 16 * tpr) tpr = 1024;
   int nv = 1;
-  while (nv * tpr < units) nv *= 2;
+  while (nv * tpr < units) nv = nv == 3 ? 4 : nv == 6 ? 8 : nv == 12 ? 16 : nv + (nv + 1) / 2;
   return {tpr, nv};
 }
 
@@ -287,12 +305,20 @@ static int launch_nv(const RowArgs& a, int nv, cudaStream_t st) {
     switch (nv) {
       case 1: return launch_row_kernel<KIND, TPR, 1, NORM>(a, st);
       case 2: return launch_row_kernel<KIND, TPR, 2, NORM>(a, st);
+      case 3: return launch_row_kernel<KIND, TPR, 3, NORM>(a, st);
       case 4: return launch_row_kernel<KIND, TPR, 4, NORM>(a, st);
       default: break;
     }
-    if constexpr (TPR > 8) return nv == 8 ? launch_row_kernel<KIND, TPR, 8, NORM>(a, st)
-                                          : launch_row_kernel<KIND, TPR, 16, NORM>(a, st);
-    else return sdb_fail(B200_ERR_SHAPE, "int8 rows: no such shape");  // 8 lanes hold at most 32 groups
+    if constexpr (TPR > 8) {
+      switch (nv) {
+        case 6: return launch_row_kernel<KIND, TPR, 6, NORM>(a, st);
+        case 8: return launch_row_kernel<KIND, TPR, 8, NORM>(a, st);
+        case 12: return launch_row_kernel<KIND, TPR, 12, NORM>(a, st);
+        case 16: return launch_row_kernel<KIND, TPR, 16, NORM>(a, st);
+        default: break;
+      }
+    }
+    return sdb_fail(B200_ERR_SHAPE, "int8 rows: no such shape");  // 8 lanes hold at most 32 groups
   }
 }
 template <bool NORM, int KIND>

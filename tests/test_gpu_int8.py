@@ -68,7 +68,9 @@ def _hard_rows(rows, k, seed):
 
 
 ROW_SHAPES = [(1, 16), (1, 2048), (1, 6144), (3, 48), (5, 1040), (21, 2032), (33, 4096), (23, 8208), (4, 32784),
-              (2, 65536), (1500, 144), (4099, 1152), (20011, 128), (10007, 16), (9601, 112), (40, 20000)]
+              (2, 65536), (1500, 144), (4099, 1152), (20011, 128), (10007, 16), (9601, 112), (40, 20000),
+              (9000, 96), (2500, 272), (2500, 384), (3500, 704), (3001, 1392), (1500, 2400), (1200, 5648), (300, 12304),
+              (70, 49168)]
 
 
 @pytest.mark.parametrize("rows,k", ROW_SHAPES)
