@@ -173,6 +173,25 @@ def load(path: str | None = None) -> C.CDLL:
         return lib
 
 
+_int8_ops = None
+
+
+def int8_ops():
+    """The extension module of the int8 operators, bound (once) to the library's entry points."""
+    global _int8_ops
+    if _int8_ops is None:
+        lib = load()
+        try:
+            from . import _int8_ops as ops
+        except ImportError as e:
+            raise RuntimeError(f"{_build.OPS} does not load ({e}): build it with `python -m strands_decider_b200.build`") \
+                from e
+        ops.bind(*(C.cast(getattr(lib, name), C.c_void_p).value
+                   for name in ("b200_quantize_act_int8", "b200_rmsnorm_int8", "b200_linear_int8")))
+        _int8_ops = ops
+    return _int8_ops
+
+
 def exported_symbols() -> list[str]:
     return sorted(_SIGS)
 

@@ -5,6 +5,9 @@
 Each .cu in csrc/ is compiled for sm_100a only (`-gencode arch=compute_100a,code=sm_100a`)
 as relocatable device code, then device-linked into one shared library. Rebuilds only
 when a source or header is newer than the library (or with --force).
+
+csrc/int8_torch.cpp becomes the Python extension module _int8_ops.so beside this file: host code
+over torch's headers, which takes the library's entry points by address and links nothing of it.
 """
 
 from __future__ import annotations
@@ -15,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +28,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libstrands_b200.so")
 OBJDIR = os.path.join(PKG, "_build")
+OPS_SRC = os.path.join(CSRC, "int8_torch.cpp")
+OPS = os.path.join(PKG, "_int8_ops.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
@@ -52,7 +58,29 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in _inputs())
 
 
+def build_ops(force: bool = False) -> str:
+    """The extension module of the int8 operators' Python calls."""
+    inputs = [OPS_SRC, os.path.join(INCLUDE, "strands_b200.h"), __file__]
+    if not force and os.path.exists(OPS) and all(os.path.getmtime(p) <= os.path.getmtime(OPS) for p in inputs):
+        return OPS
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    tmp = OPS + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}",
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           OPS_SRC, "-o", tmp, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {os.path.basename(OPS_SRC)}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, OPS)
+    return OPS
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False, extra: list[str] | None = None) -> str:
+    build_ops(force)
     if not force and up_to_date():
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)

@@ -550,6 +550,33 @@ def test_python_operators_refuse_before_launching():
                 lambda: int8.linear(q, s, w, out, epilogue="swiglu")):
         with pytest.raises(ValueError):
             bad()
+    # what only a later argument shows: another device, type, stride or number of outputs
+    pw = W.PackedWeight
+    wide = torch.zeros(256, 64, dtype=torch.int8, device="cuda")
+    act = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    buf = torch.zeros(4, 64, dtype=torch.uint8, device="cuda")
+    for bad in (lambda: int8.quantize_act(act, lo=torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")[:, ::2]),
+                lambda: int8.quantize_act(act, lo=torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")[:, :64]),
+                lambda: int8.quantize_act(act.to_sparse()), lambda: int8.quantize_act(act, lo=act.cpu()),
+                lambda: int8.rmsnorm(x, torch.zeros(128, device="cuda")[::2], 1e-6),
+                lambda: int8.rmsnorm(x, torch.zeros(64), 1e-6),
+                lambda: int8.rmsnorm(x, torch.zeros(64, device="cuda"), 1e-6, delta=x[:3]),
+                lambda: int8.rmsnorm(x, torch.zeros(64, device="cuda"), 1e-6, delta=x, resid_out=x.to(torch.bfloat16)),
+                lambda: int8.linear(q, s, pw("int8", 128, 64, wide[::2], row_scale=w.row_scale), out),
+                lambda: int8.linear(q, s, pw("int8", 128, 64, w.data.cpu(), row_scale=w.row_scale), out),
+                lambda: int8.linear(q, s, pw("int8", 128, 64, w.data.float(), row_scale=w.row_scale), out),
+                lambda: int8.linear(q, s, pw("int8", 128, 64, w.data, row_scale=w.row_scale[:64]), out),
+                lambda: int8.linear(q, s, pw("int8", 128, 64, w.data), out),
+                lambda: int8.linear(q, s, w, out, n_valid=1 << 40), lambda: int8.linear(q, s, w, out, n_valid=64),
+                lambda: int8.linear(q, s, w, act, epilogue="swiglu", lo=act),
+                lambda: int8.linear(q, s, w, act, epilogue="swiglu", lo=act.float()),
+                lambda: int8.linear(q, s, w, act, epilogue="swiglu", lo=buf.cpu())):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: int8.linear(q, s, w, out, n_valid=1.5), lambda: int8.rmsnorm(x, x[0], None),
+                lambda: int8.linear(q, s, w, None)):
+        with pytest.raises(TypeError):
+            bad()
     for bad in (lambda: int8.quantize_act(x[:, :40]), lambda: int8.quantize_act(x[:0]),
                 lambda: int8.rmsnorm(x, torch.zeros(64, device="cuda"), -1.0),
                 lambda: int8.linear(q[:, :48], s, w, out)):

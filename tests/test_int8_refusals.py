@@ -143,3 +143,26 @@ def test_python_operators_refuse_cpu_tensors_and_wrong_types():
         int8.rmsnorm(x, torch.zeros(64), 1e-6)
     with pytest.raises(ValueError, match="CUDA"):
         int8.linear(x.to(torch.int8), torch.ones(2), w, torch.zeros(2, 128))
+
+
+def test_python_operators_refuse_what_is_not_a_cuda_tensor(lib):
+    from strands_decider_b200 import _lib, int8
+    from strands_decider_b200.weights import PackedWeight
+
+    x, s, w = torch.zeros(2, 16), torch.zeros(2), torch.zeros(16)
+    q, out = torch.zeros(2, 16, dtype=torch.int8), torch.zeros(2, 8)
+    pw = PackedWeight("int8", 8, 16, torch.zeros(8, 16, dtype=torch.int8), row_scale=torch.zeros(8))
+    for bad in (lambda: int8.quantize_act(x), lambda: int8.rmsnorm(x, w, 1e-6), lambda: int8.linear(q, s, pw, out),
+                lambda: int8.linear(q, s, PackedWeight("int8", 8, 16, pw.data), out),
+                lambda: int8.linear(q, s, pw, out, epilogue="gelu")):
+        with pytest.raises(ValueError):
+            bad()
+    ops = _lib.int8_ops()
+    for bad in (lambda: ops.quantize_act(x, None, q, s, 0), lambda: ops.rmsnorm(x, w, 1e-6, None, None, q, s, 0),
+                lambda: ops.linear(q, s, pw.data, pw.row_scale, out, None, 8, 16, 8, 0, 0)):
+        with pytest.raises(ValueError, match="CUDA tensors only"):
+            bad()
+    for bad in (lambda: ops.quantize_act(x.numpy(), None, q, s, 0), lambda: ops.linear(None, *[x] * 10),
+                lambda: ops.rmsnorm(x), lambda: ops.bind(1, 2), lambda: ops.bind("a", 2, 3)):
+        with pytest.raises(TypeError):
+            bad()
