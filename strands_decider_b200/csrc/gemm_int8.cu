@@ -530,8 +530,16 @@ constexpr int I8S_OP_W = 128 * I8_BK;
 constexpr int I8S_MAX_STAGES = 12;
 constexpr int I8S_RING = 220 * 1024;       // bytes of stages: one CTA per SM
 constexpr int I8S_RING_HALF = 104 * 1024;  // two CTAs per SM
+// Columns of tensor memory: the two accumulators.
+__host__ __device__ constexpr int i8s_cols(int bt) { return bt <= 32 ? 64 : bt <= 64 ? 128 : 256; }
+// Shared memory: what the CTA uses, and at least as large a share of the SM's 228 KB (of which each
+// CTA costs 1 KB more) as its columns are of 512. So whatever CTAs of this kernel an SM takes in, of
+// several streams too, its tensor memory serves them all, and no cluster waits for columns that
+// another holds while it waits for the first.
 constexpr int i8s_smem(int stages, int bt) {
-  return 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (4 * I8S_MAX_STAGES + 1) * 8 + 16;
+  const int used = 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (4 * I8S_MAX_STAGES + 1) * 8 + 16;
+  const int share = 228 * 1024 / 512 * i8s_cols(bt) - 1024;
+  return used > share ? used : share;
 }
 
 __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
@@ -564,7 +572,7 @@ __global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
   const int rank = blockIdx.x % SPLIT, n0 = blockIdx.x / SPLIT * 128, t0 = blockIdx.y * bt;
   const int nk = (a.k + I8_BK - 1) / I8_BK;
   const int kb0 = int(int64_t(rank) * nk / SPLIT), kb1 = int(int64_t(rank + 1) * nk / SPLIT);
-  const uint32_t cols = bt <= 32 ? 32 : bt <= 64 ? 64 : 128;  // of one accumulator
+  const uint32_t cols = i8s_cols(bt) / 2;  // of one accumulator
 
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2 * stages; ++b) {
@@ -1022,9 +1030,8 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   // ring (96 x 12288 x 2048: 8.9 us against 11.7).
   const int stage = I8S_OP_W + a.bt * I8_BK, nkb = (nk + split - 1) / split;
   const bool half = tiles * split > sm_count() || 3 * (I8S_RING_HALF / stage) >= 2 * nkb;
-  // Two stages at least, for the sums' way through shared memory; three with 256 columns of TMEM, so
-  // that no more CTAs fit on an SM than its TMEM serves.
-  a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(a.bt > 64 ? 3 : 2, nkb)});
+  // Two stages at least: the sums take their room.
+  a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(2, nkb)});
   switch (split) {
     case 1: return launch_i8_cluster<EP, LO, 1>(a, n_tiles, m_tiles, st);
     case 2: return launch_i8_cluster<EP, LO, 2>(a, n_tiles, m_tiles, st);
