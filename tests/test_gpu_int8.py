@@ -524,6 +524,35 @@ def test_mlp_captured_replayed_and_on_two_streams():
         assert torch.equal(buf, _mlp(x2.clone(), d2, p, b))
 
 
+def test_mlps_of_four_threads_on_streams_of_their_own():
+    """Calls from several host threads at once, launches of every kind beside one another on the SMs."""
+    import threading
+
+    sets = [_mlp_setup(m, hidden=1024, inter=2048) for m in (7, 30, 130, 1400)]
+    want = [_mlp(x.clone(), d, p, b).clone() for p, b, x, d in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        try:
+            p, b, x, d = sets[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(40):
+                    got = _mlp(x.clone(), d, p, b)
+                    if not torch.equal(got, want[i]):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001 - reported below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
+
+
 def test_python_operators_refuse_before_launching():
     from strands_decider_b200 import _lib, int8
     from strands_decider_b200 import weights as W
