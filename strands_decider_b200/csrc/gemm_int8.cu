@@ -1026,10 +1026,12 @@ static int launch_i8_split(I8Args a, cudaStream_t st) {
   while (split < (a.bt <= 32 ? 8 : 4) && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
   // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 300
   // x 12288 x 2048 17.8 -> 13.2 us), or when that ring holds most of the CTA's K anyway (the next
-  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 12.1 -> 7.7 us); else the deeper
-  // ring (96 x 12288 x 2048: 8.9 us against 11.7).
+  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 12.1 -> 7.7 us), or for clusters of
+  // 8 on most SMs, which else wait for one another's end (32 x 2048 x 8192 13.2 -> 8.7 us; on 64 SMs,
+  // 1024 x 8192, 6.6 : 6.9); else the deeper ring (96 x 12288 x 2048: 8.9 us against 11.7).
   const int stage = I8S_OP_W + a.bt * I8_BK, nkb = (nk + split - 1) / split;
-  const bool half = tiles * split > sm_count() || 3 * (I8S_RING_HALF / stage) >= 2 * nkb;
+  const bool half = tiles * split > sm_count() || 3 * (I8S_RING_HALF / stage) >= 2 * nkb ||
+                    (split == 8 && 2 * tiles * split > sm_count());
   // Two stages at least: the sums take their room.
   a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(2, nkb)});
   switch (split) {
@@ -1068,10 +1070,25 @@ static int dispatch_i8_reg(const I8Args& a, cudaStream_t st) {
   }
 }
 
+// Whether the register kernel takes the product. It starts sooner, but loads through registers, and
+// few CTAs share a long K: beyond some weight bytes, or some K, the split kernel's copies are faster.
+// us, registers : split - 1 token, 12288 x 2048 SwiGLU 6.0 : 7.2, 24576 x 1024 6.1 : 7.0, 32768 x 2048
+// store 15.0 : 12.4, 8192 x 3088 residual 7.1 : 8.4, 1024 x 16384 10.3 : 7.3, 1024 x 8192 4.2 : 4.9;
+// SwiGLU of K 4096, 2048 outputs 5.4 : 4.6, 6144 9.4 : 8.0, K 3088 8.5 : 8.5; 16 tokens, SwiGLU 12288 x
+// 1024 4.5 : 4.7, 8192 x 2048 7.4 : 6.6, 4096 x 3088 8.3 : 6.7, 4096 x 2048 5.1 : 5.6; residual 8192 x
+// 3088 8.6 : 10.1, 32768 x 1024 10.1 : 8.0.
+static bool i8_few_tokens(const I8Args& a, bool swiglu) {
+  if (a.m > I8R_MAX_M) return false;
+  const double bytes = double(a.o.n_valid) * a.k;
+  if (swiglu) return a.m <= 8 ? a.k < 4096 && bytes <= 32e6 : a.k <= 2048 && bytes <= 14e6;
+  return a.k < 16384 && bytes <= (a.m <= 8 ? 32e6 : 26e6);
+}
+
 template <int EP>
 static int launch_int8(const I8Args& a, cudaStream_t st) {
-  if (a.m <= 8) return dispatch_i8_reg<EP, 1>(a, st);
-  if (a.m <= I8R_MAX_M) return dispatch_i8_reg<EP, 2>(a, st);
+  if (i8_few_tokens(a, EP == B200_EP_SWIGLU)) {
+    return a.m <= 8 ? dispatch_i8_reg<EP, 1>(a, st) : dispatch_i8_reg<EP, 2>(a, st);
+  }
   // Single CTAs while each 128 x 128 tile has an SM (1021 x 2048 x 6144: 17.8 us, pairs 25). With two
   // of them to an SM, pairs if one round of them does (2000 x 2048 x 6144: 27.2 us against 46.2; 300 x
   // 8224 x 2048: 11.7 : 13.1), unless K is short, where two CTAs hide each other's set-up and outputs

@@ -189,7 +189,8 @@ SHAPES = [(1, 1, 16), (1, 130, 64), (2, 2048, 2048), (7, 1000, 144), (8, 96, 820
           (17, 640, 2048), (31, 33, 48), (33, 129, 6144), (64, 1153, 528), (65, 256, 4112), (96, 8224, 256),
           (127, 384, 1024), (129, 127, 272), (200, 2048, 2032), (255, 600, 2064), (257, 520, 128), (511, 1025, 400),
           (1021, 2048, 2048), (1290, 2040, 1040), (2050, 4200, 336), (2050, 4201, 144),
-          (4099, 2600, 1040), (9001, 1290, 144)]
+          (4099, 2600, 1040), (9001, 1290, 144),
+          (1, 20000, 2048), (3, 130, 16384), (8, 1000, 65536), (9, 16, 16400), (12, 9000, 3088), (16, 2048, 20480)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -210,7 +211,7 @@ def test_linear_store_and_residual(m, n, k):
 
 SWIGLU_SHAPES = [(1, 128, 16), (1, 12288, 256), (5, 256, 144), (13, 1152, 2048), (16, 128, 1040), (24, 640, 528),
                  (96, 1024, 2048), (130, 384, 400), (300, 2432, 1024), (600, 5504, 1040), (500, 5504, 1040), (1030, 1280, 272), (2050, 4224, 160),
-                 (3333, 3200, 144)]
+                 (3333, 3200, 144), (1, 128, 4096), (3, 384, 16384), (8, 20096, 2048), (9, 256, 2064), (16, 12288, 2048)]
 
 
 @pytest.mark.parametrize("m,n,k", SWIGLU_SHAPES)
