@@ -522,7 +522,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 // At these sizes a launch is a chain of latencies. 96 x 8224 x 2048 (clusters of 2), 8.4 us in a row
 // of launches, of which one takes 7.2: 0.5 set-up, 3 until the last MMA (8 k-blocks of 28 KB),
 // 0.4 sums to shared memory, 0.7 cluster barrier, 1.3 outputs, 0.8 last barrier.
-// Warps per CTA. Alone on its SM a CTA takes 16 (1021 x 2048 x 2048: 10.3 us against 11.3); CTAs of
+// Warps per CTA. Without a cluster a CTA takes 16 (1021 x 2048 x 2048: 10.3 us against 11.3), with
+// registers for two of them an SM (1 x 32768 x 2048 residual: 12.8 us against 17.1); CTAs of
 // a cluster take 8, and the next launch's clusters find room beside them (32 x 2048 x 6144 on
 // clusters of 8: 7.7 us against 12.6).
 constexpr int i8s_warps(int split) { return split == 1 ? 16 : 8; }
@@ -552,7 +553,7 @@ __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
 __device__ __forceinline__ int4 add4(int4 a, int4 b) { return make_int4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
 template <int EP, bool LO, int SPLIT>
-__global__ void __launch_bounds__(32 * i8s_warps(SPLIT), 1)
+__global__ void __launch_bounds__(32 * i8s_warps(SPLIT), SPLIT == 1 ? 2 : 1)
     gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                          const I8Args a) {
   extern __shared__ uint8_t i8_smem_raw[];
@@ -1076,10 +1077,13 @@ static int dispatch_i8_reg(const I8Args& a, cudaStream_t st) {
 // store 15.0 : 12.4, 8192 x 3088 residual 7.1 : 8.4, 1024 x 16384 10.3 : 7.3, 1024 x 8192 4.2 : 4.9;
 // SwiGLU of K 4096, 2048 outputs 5.4 : 4.6, 6144 9.4 : 8.0, K 3088 8.5 : 8.5; 16 tokens, SwiGLU 12288 x
 // 1024 4.5 : 4.7, 8192 x 2048 7.4 : 6.6, 4096 x 3088 8.3 : 6.7, 4096 x 2048 5.1 : 5.6; residual 8192 x
-// 3088 8.6 : 10.1, 32768 x 1024 10.1 : 8.0.
+// 3088 8.6 : 10.1, 32768 x 1024 10.1 : 8.0. With more feature tiles than two a SM, where the split
+// kernel takes more than a round, 1 token 98304 x 2048 30.6 : 36.2, 49152 x 1024 10.0 : 12.5, 49152 x
+// 6144 64 : 57; 16 tokens 98304 x 2048 39.8 : 37.6.
 static bool i8_few_tokens(const I8Args& a, bool swiglu) {
   if (a.m > I8R_MAX_M) return false;
   const double bytes = double(a.o.n_valid) * a.k;
+  if (a.m <= 8 && a.o.n_valid > 256 * sm_count()) return a.k <= 2048;
   if (swiglu) return a.m <= 8 ? a.k < 4096 && bytes <= 32e6 : a.k <= 2048 && bytes <= 14e6;
   return a.k < 16384 && bytes <= (a.m <= 8 ? 32e6 : 26e6);
 }
@@ -1094,12 +1098,14 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   // 8224 x 2048: 11.7 : 13.1), unless K is short, where two CTAs hide each other's set-up and outputs
   // (200 x 16384 x 512: 9.2 : 7.5; at K = 1024 both are within 8 %). Where pairs would take two
   // rounds, single CTAs (300 x 12288 x 2048: 13.0 us against 17.7). Pairs beyond (512 x 12288 x 2048:
-  // 18.6 us against 22).
+  // 18.6 us against 22), but not for 32 tokens or fewer, of which a pair's tile would be almost empty
+  // (32 x 98304 x 2048: 37.8 us in single CTAs, several rounds of them, against 43.6; 64 tokens 41 : 43,
+  // 100 tokens 46 : 44).
   const int sms = sm_count();
   const int64_t tiles = int64_t((a.o.n_valid + 127) / 128) * ((a.m + 127) / 128);
   const int64_t pair_tiles = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
   constexpr bool SW = EP == B200_EP_SWIGLU;
-  if (tiles <= sms || (tiles <= 2 * sms && (2 * pair_tiles > sms || a.k <= 1024))) {
+  if (tiles <= sms || a.m <= 32 || (tiles <= 2 * sms && (2 * pair_tiles > sms || a.k <= 1024))) {
     if constexpr (SW) {
       if (a.o.lo_offset) return launch_i8_split<EP, true>(a, st);
     }
