@@ -517,11 +517,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 //   warp 0  TMA ring; warps 1 and 2  MMAs; then all warps drain the accumulators and finish outputs.
 // Two threads issue MMAs. To issue one costs a thread 35 to 40 ns, more than the tensor cores need for
 // 128 tokens or fewer, so each of two takes every second k-block, with an accumulator of its own (the
-// sums are whole numbers: their order changes nothing). 96 x 8224 x 2048 8.4 us, with one issuer 9.1;
-// 1021 x 2048 x 6144 17.8 : 21.2. (Half of every k-block each: 8.8 and 18.4 us.)
-// At these sizes a launch is a chain of latencies. 96 x 8224 x 2048 (clusters of 2), 8.4 us in a row
+// sums are whole numbers: their order changes nothing). 96 x 8224 x 2048 on clusters of 2 8.4 us, with
+// one issuer 9.1; 1021 x 2048 x 6144 17.8 : 21.2. (Half of every k-block each: 8.8 and 18.4 us.)
+// At these sizes a launch is a chain of latencies. 96 x 8224 x 2048 on clusters of 2, 8.4 us in a row
 // of launches, of which one takes 7.2: 0.5 set-up, 3 until the last MMA (8 k-blocks of 28 KB),
-// 0.4 sums to shared memory, 0.7 cluster barrier, 1.3 outputs, 0.8 last barrier.
+// 0.4 sums to shared memory, 0.7 cluster barrier, 1.3 outputs, 0.8 last barrier. In two token tiles
+// of 48 instead, without a cluster, it takes 7.6.
 // Warps per CTA. Without a cluster a CTA takes 16 (1021 x 2048 x 2048: 10.3 us against 11.3), with
 // registers for two of them an SM (1 x 32768 x 2048 residual: 12.8 us against 17.1); CTAs of
 // a cluster take 8, and the next launch's clusters find room beside them (32 x 2048 x 6144 on
@@ -1016,15 +1017,23 @@ static int launch_i8_cluster(const I8Args& a, int n_tiles, int m_tiles, cudaStre
 template <int EP, bool LO>
 static int launch_i8_split(I8Args a, cudaStream_t st) {
   const int nk = (a.k + I8_BK - 1) / I8_BK, n_tiles = (a.o.n_valid + 127) / 128;
-  int m_tiles = (a.m + 127) / 128;
+  // Tokens of a tile, at most: 128, or with 16 k-blocks or fewer the fewest of 32, 64 and 128 whose
+  // tiles each have an SM. Where K is short, splitting the tokens is cheaper than splitting K, whose
+  // sums cross the cluster (128 x 1024 x 1024 4.6 us against 5.7, 128 x 2048 x 2048 6.6 : 7.3, 96 x
+  // 8224 x 2048 7.6 : 8.3; K 6144, 200 x 2048: 14.4 : 10.2).
+  const bool shallow = nk <= 16;
+  int most = shallow ? 32 : 128;
+  while (most < 128 && int64_t(n_tiles) * ((a.m + most - 1) / most) > sm_count()) most *= 2;
+  int m_tiles = (a.m + most - 1) / most;
   a.bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
   m_tiles = (a.m + a.bt - 1) / a.bt;
   const int tiles = n_tiles * m_tiles;
   // K split over a cluster while SMs would idle and every CTA has two k-blocks. Clusters of 8 only
   // for at most 32 tokens: they wait longest for their SMs, and each of their CTAs reads as many sums
   // as one of 4 (2048 x 6144: 32 tokens 7.7 us against 8.3 on clusters of 4, 128 tokens 15.3 : 9.4).
+  // At most 2 with 16 k-blocks or fewer (64 x 2048 x 2048 in tiles of 32: 5.8 us against 6.7 on 4).
   int split = 1;
-  while (split < (a.bt <= 32 ? 8 : 4) && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
+  while (split < (shallow ? 2 : a.bt <= 32 ? 8 : 4) && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
   // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 300
   // x 12288 x 2048 17.8 -> 13.2 us), or when that ring holds most of the CTA's K anyway (the next
   // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 12.1 -> 7.7 us), or for clusters of
