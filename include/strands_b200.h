@@ -224,6 +224,33 @@ int b200_rmsnorm_int8(const float* x, int32_t ldx, const void* delta, int32_t de
 int b200_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
                      const b200_linear_out* out, b200_stream stream);
 
+/* ---------------------------------------------------------------- launch plans
+ * How a linear would be launched on a device of `sms` SMs: host arithmetic for tests and profiles;
+ * nothing is read through the pointers or launched, and arguments are refused as by the linear. */
+enum b200_linear_kernel {
+  B200_KERNEL_OTHER = 0,      /* one of b200_linear's kernels without a cluster */
+  B200_KERNEL_BF16_PAIR = 1,  /* b200_linear, bf16 weights: CTA pairs */
+  B200_KERNEL_INT8_REG = 2,   /* b200_linear_int8: weights through registers */
+  B200_KERNEL_INT8_SPLIT = 3, /* a CTA or cluster of K ranges per tile */
+  B200_KERNEL_INT8_PAIR = 4   /* CTA pairs */
+};
+
+/* 0 where a kernel has no such thing (OTHER: everything; INT8_REG: all but kernel and cluster). */
+typedef struct b200_launch_plan {
+  int32_t kernel;                /* enum b200_linear_kernel */
+  int32_t ctas, cluster, threads; /* CTAs, CTAs per cluster, threads per CTA */
+  int32_t smem_bytes, tmem_cols; /* shared memory and tensor memory columns a CTA asks for */
+  int32_t tile_n, tile_m, tiles; /* outputs and tokens of a tile, tiles */
+  int32_t stages, k_blocks;      /* operand ring depth, and its most fills for one tile */
+  int32_t group_tiles;           /* pairs: output tiles whose weights are kept in L2 together */
+} b200_launch_plan;
+
+int b200_linear_plan(const uint16_t* x_hi, const uint16_t* x_lo, int32_t m, int32_t k, int32_t ldx,
+                     const b200_qweight* w, const b200_linear_out* out, int32_t sms, b200_launch_plan* plan);
+/* sms = 0: the current device, its own number of CTA pairs at once included (else sms / 2). */
+int b200_linear_int8_plan(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx,
+                          const b200_qweight* w, const b200_linear_out* out, int32_t sms, b200_launch_plan* plan);
+
 /* ---------------------------------------------------------------- ragged batches, prefix cache */
 typedef struct b200_seqs {
   int32_t n_seqs;

@@ -46,6 +46,14 @@ class LinearOut(C.Structure):
                 ("lo_offset", C.c_int64), ("lo_format", C.c_int32)]
 
 
+KERNEL_OTHER, KERNEL_BF16_PAIR, KERNEL_INT8_REG, KERNEL_INT8_SPLIT, KERNEL_INT8_PAIR = range(5)
+
+
+class LaunchPlan(C.Structure):
+    _fields_ = [(name, C.c_int32) for name in ("kernel", "ctas", "cluster", "threads", "smem_bytes", "tmem_cols",
+                                               "tile_n", "tile_m", "tiles", "stages", "k_blocks", "group_tiles")]
+
+
 class Seqs(C.Structure):
     _fields_ = [("n_seqs", C.c_int32), ("n_tokens", C.c_int32), ("max_len", C.c_int32),
                 ("cu_seqlens", C.c_void_p), ("prefix_slot", C.c_void_p), ("save_slot", C.c_void_p)]
@@ -136,6 +144,9 @@ _SIGS = {
     "b200_quantize_act_int8": ([_P, _P, _I, _I, _I, _I, _P, _I, _P, _P], C.c_int),
     "b200_rmsnorm_int8": ([_P, _I, _P, _I, _I, _P, _I, _I, _I, _P, C.c_float, _P, _I, _P, _P], C.c_int),
     "b200_linear_int8": ([_P, _P, _I, _I, _I, C.POINTER(QWeight), C.POINTER(LinearOut), _P], C.c_int),
+    "b200_linear_plan": ([_P, _P, _I, _I, _I, C.POINTER(QWeight), C.POINTER(LinearOut), _I, C.POINTER(LaunchPlan)], C.c_int),
+    "b200_linear_int8_plan": ([_P, _P, _I, _I, _I, C.POINTER(QWeight), C.POINTER(LinearOut), _I, C.POINTER(LaunchPlan)],
+                              C.c_int),
     "b200_decide_readout": ([_P, _I, _P, C.c_float, C.POINTER(Readout), C.POINTER(DecideArgs), _I, _P], C.c_int),
     "b200_model_create": ([C.POINTER(ModelConfig), C.POINTER(C.c_void_p)], C.c_int),
     "b200_model_destroy": ([_P], C.c_int),

@@ -518,6 +518,19 @@ int encode_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64
 // bytes, so cols must be a multiple of 8. Defined in gemm.cu.
 int encode_store_tile(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows, int box_cols);
 
+// Shared memory of clusters with tensor memory. An SM takes a CTA in by its shared memory, threads and
+// registers; its tensor memory columns a CTA then asks for itself, and waits while others hold them. A
+// CTA of a cluster that holds columns ends only after the others of its cluster have theirs: two
+// clusters that met on two SMs, each with its columns on one of them, would wait for ever. So what
+// CTAs of such kernels an SM has room for, of several streams too, must find columns for all of them.
+// A kernel that takes all 512 asks for at least kWholeTmemSmem, beside which no CTA of kClusterSmemMin
+// has room, the least that any of these kernels asks for; those that take fewer share as
+// gemm_int8.cu's split kernel does. (A CTA without a cluster that waits for columns holds none.)
+constexpr int kSmSmem = 228 * 1024;         // of an SM
+constexpr int kCtaSmem = 1024;              // taken by each CTA beside its own
+constexpr int kClusterSmemMin = 36 * 1024;
+constexpr int kWholeTmemSmem = kSmSmem - 2 * kCtaSmem - kClusterSmemMin + 16;
+
 // Kernel attributes (such as the dynamic shared-memory limit) are per device, and one process
 // may drive several GPUs from several host threads. A DeviceOnce runs a set-up step once per
 // device, under its lock, with that device current; the step returns a B200 status and is

@@ -414,7 +414,9 @@ struct Gemm2Smem {
   static constexpr int STAGE = A_STAGE + B_BYTES + B8_BYTES;
   static constexpr int STAGES = GEMM2_STAGES;
   static constexpr int BARS = 2 * STAGES + 4;
-  static constexpr int TOTAL = STAGES * STAGE + 1024 + BARS * 8 + 16;
+  static constexpr int USED = STAGES * STAGE + 1024 + BARS * 8 + 16;
+  // one plane uses 129 KB: more is asked for so that no other cluster's CTA shares the SM
+  static constexpr int TOTAL = USED > kWholeTmemSmem ? USED : kWholeTmemSmem;
 };
 
 template <int EP, int PL>
@@ -1182,6 +1184,30 @@ static int dispatch_ep(const CUtensorMap& map, const CUtensorMap& map_lo, const 
   }
 }
 
+// The CTA-pair kernel's launch where the device holds `pairs` pairs at once.
+template <int PL>
+static b200_launch_plan plan_pair(const GemmArgs& a, int pairs) {
+  // Weight bytes of all column tiles beyond what L2 keeps alongside the activation stream
+  // (about 48 MB here: the 126 MB L2 holds a line in each die's half when both dies read it)
+  // -> groups of column tiles of at most about 40 MB each.
+  const int n_tiles_n = a.w.n / 256;
+  const double tile_bytes = 256.0 * a.k * (PL == PL_LO8 ? 3 : 2);
+  const int groups = n_tiles_n * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles_n * tile_bytes / 40e6));
+  b200_launch_plan p = {};
+  p.kernel = B200_KERNEL_BF16_PAIR;
+  p.tile_n = p.tile_m = 256;
+  p.tiles = n_tiles_n * ((a.m + 255) / 256);
+  p.ctas = 2 * std::min(p.tiles, pairs);
+  p.cluster = 2;
+  p.threads = GEMM2_THREADS;
+  p.smem_bytes = Gemm2Smem<PL>::TOTAL;
+  p.tmem_cols = 512;
+  p.stages = GEMM2_STAGES;
+  p.k_blocks = a.k / GEMM_BK;
+  p.group_tiles = (n_tiles_n + groups - 1) / groups;
+  return p;
+}
+
 // The CTA-pair kernel: bf16 weight copies, 256 x 256 tiles, at least one tile per pair.
 template <int EP, int PL>
 static int launch_pair(const CUtensorMap& map, const CUtensorMap& map_lo, const CUtensorMap& map_b,
@@ -1207,19 +1233,12 @@ static int launch_pair(const CUtensorMap& map, const CUtensorMap& map_lo, const 
   if (r != B200_OK) return r;
   int dev = 0;
   SDB_CUDA(cudaGetDevice(&dev));
-  const int max_pairs = max_pairs_dev[dev];
+  const b200_launch_plan p = plan_pair<PL>(a, max_pairs_dev[dev]);
   GemmArgs args = a;
   args.ksplit = 1;
-  // Weight bytes of all column tiles beyond what L2 keeps alongside the activation stream
-  // (about 48 MB here: the 126 MB L2 holds a line in each die's half when both dies read it)
-  // -> groups of column tiles of at most about 40 MB each.
-  const int n_tiles_n = a.w.n / 256;
-  const double tile_bytes = 256.0 * a.k * (PL == PL_LO8 ? 3 : 2);
-  const int groups = n_tiles_n * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles_n * tile_bytes / 40e6));
-  args.ngroup = (n_tiles_n + groups - 1) / groups;
-  const int units = n_tiles_n * ((a.m + 255) / 256);
-  SDB_CUDA(launch_pdl(gemm_pair_kernel<EP, PL>, dim3(2 * std::min(units, max_pairs)), dim3(GEMM2_THREADS), smem, st,
-                      map, map_lo, map_b, map_b8, args));
+  args.ngroup = p.group_tiles;
+  SDB_CUDA(launch_pdl(gemm_pair_kernel<EP, PL>, dim3(p.ctas), dim3(GEMM2_THREADS), smem, st, map, map_lo, map_b, map_b8,
+                      args));
   return B200_OK;
 }
 
@@ -1234,9 +1253,7 @@ static int dispatch_pair(const CUtensorMap& map, const CUtensorMap& map_lo, cons
 }
 
 // Pairs pay off once every pair has a whole 256 x 256 tile.
-static bool pair_path(const GemmArgs& a) {
-  return (a.w.n / 256) * ((a.m + 255) / 256) >= sm_count() / 2;
-}
+static bool pair_path(const GemmArgs& a, int sms) { return (a.w.n / 256) * ((a.m + 255) / 256) >= sms / 2; }
 
 template <int PL>
 static int dispatch_fmt(const CUtensorMap& map, const CUtensorMap& map_lo, const CUtensorMap& map_b, const GemmArgs& a,
@@ -1358,7 +1375,7 @@ extern "C" int b200_linear(const uint16_t* x_hi, const uint16_t* x_lo, int32_t m
   }
   if (w->format == B200_W_BF16) {  // the weight tile streams through TMA as [n, k] bf16, one box per N tile
     if (reinterpret_cast<uintptr_t>(w->data) & 15) return sdb_fail(B200_ERR_SHAPE, "b200_linear: bf16 W unaligned");
-    if (pair_path(a)) {  // each CTA of a pair loads 128 of the tile's 256 weight rows
+    if (pair_path(a, sm_count())) {  // each CTA of a pair loads 128 of the tile's 256 weight rows
       if (int rc = make_act_map(&map_b, reinterpret_cast<const uint16_t*>(w->data), w->n, k, k, 128)) return rc;
       return x_lo ? dispatch_pair<PL_SPLIT>(map, map_lo, map_b, map_b, a, st)
                   : dispatch_pair<PL_ONE>(map, map_lo, map_b, map_b, a, st);
@@ -1371,6 +1388,17 @@ extern "C" int b200_linear(const uint16_t* x_hi, const uint16_t* x_lo, int32_t m
   return x_lo ? dispatch_fmt<PL_SPLIT>(map, map_lo, map_b, a, st) : dispatch_fmt<PL_ONE>(map, map_lo, map_b, a, st);
 }
 
+extern "C" int b200_linear_plan(const uint16_t* x_hi, const uint16_t* x_lo, int32_t m, int32_t k, int32_t ldx,
+                                const b200_qweight* w, const b200_linear_out* out, int32_t sms, b200_launch_plan* plan) {
+  if (!plan || sms <= 0) return sdb_fail(B200_ERR_ARG, "b200_linear_plan: no plan, or no SMs");
+  if (int rc = check_linear(x_hi, x_lo, m, k, ldx, w, out)) return rc;
+  GemmArgs a{*w, *out, m, k, 1};
+  *plan = {};
+  if (w->format == B200_W_BF16 && pair_path(a, sms))
+    *plan = x_lo ? plan_pair<PL_SPLIT>(a, std::max(1, sms / 2)) : plan_pair<PL_ONE>(a, std::max(1, sms / 2));
+  return B200_OK;
+}
+
 extern "C" int b200_linear_lo8(const uint16_t* x_hi, const uint8_t* x_lo8, int32_t m, int32_t k, int32_t ldx,
                                const uint16_t* w_hi, const uint8_t* w_lo8, int32_t n, const b200_linear_out* out,
                                b200_stream stream) {
@@ -1380,7 +1408,7 @@ extern "C" int b200_linear_lo8(const uint16_t* x_hi, const uint8_t* x_lo8, int32
   if (ldx % 16 != 0 || (reinterpret_cast<uintptr_t>(w_hi) & 15) || (reinterpret_cast<uintptr_t>(w_lo8) & 15))
     return sdb_fail(B200_ERR_SHAPE, "b200_linear_lo8: ldx % 16 and 16-byte aligned weight copies required");
   GemmArgs a{w, *out, m, k, 1};
-  const bool pair = pair_path(a);
+  const bool pair = pair_path(a, sm_count());
   const int bn = pair ? 128 : tile_bn(a);  // weight rows per TMA box (a pair CTA loads half a tile)
   CUtensorMap map, map_lo, map_b, map_b8;
   if (int rc = make_tile_map(&map, x_hi, false, m, k, ldx, GEMM_BM)) return rc;

@@ -13,6 +13,7 @@
 //   gemm_i8_reg_kernel    at most 16 tokens and weights of some MB: these through registers into mma.sync
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -181,6 +182,7 @@ struct I8PairSmem {
   static constexpr int BARS = 2 * STAGES + 4;
   static constexpr int TOTAL = 1024 + STAGES * STAGE + I8P_EPI_WARPS * TILES + XS + BARS * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
+  static_assert(TOTAL >= kWholeTmemSmem, "a pair that takes all tensor memory columns has the SM to itself");
 };
 
 // CW neighbouring columns (tokens) of one accumulator lane (feature), stored at p and ldo apart.
@@ -534,15 +536,16 @@ constexpr int I8S_RING = 220 * 1024;       // bytes of stages: one CTA per SM
 constexpr int I8S_RING_HALF = 104 * 1024;  // two CTAs per SM
 // Columns of tensor memory: the two accumulators.
 __host__ __device__ constexpr int i8s_cols(int bt) { return bt <= 32 ? 64 : bt <= 64 ? 128 : 256; }
-// Shared memory: what the CTA uses, and at least as large a share of the SM's 228 KB (of which each
-// CTA costs 1 KB more) as its columns are of 512. So whatever CTAs of this kernel an SM takes in, of
-// several streams too, its tensor memory serves them all, and no cluster waits for columns that
-// another holds while it waits for the first.
+// Shared memory: what the CTA uses, and at least as large a share of the SM's as its columns are of
+// 512. So whatever CTAs of this kernel an SM takes in, of several streams too, its tensor memory serves
+// them all, and no cluster waits for columns that another holds while it waits for the first; nor
+// beside a cluster kernel that takes all columns (kWholeTmemSmem).
 constexpr int i8s_smem(int stages, int bt) {
   const int used = 1024 + stages * (I8S_OP_W + bt * I8_BK) + 128 * 4 + (4 * I8S_MAX_STAGES + 1) * 8 + 16;
-  const int share = 228 * 1024 / 512 * i8s_cols(bt) - 1024;
+  const int share = kSmSmem / 512 * i8s_cols(bt) - kCtaSmem;
   return used > share ? used : share;
 }
+static_assert(i8s_smem(2, 16) >= kClusterSmemMin, "two stages of 16 tokens are the least that a CTA asks for");
 
 __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr) {
   int4 v;
@@ -935,8 +938,9 @@ static int i8_swiglu_map(CUtensorMap* map, const void* base, int blocks, int k) 
   return encode_bf16_sw128(map, base, 5, dims, strides, box);
 }
 
+// CTA pairs of a pair kernel that the current device holds at once (and the kernel's attributes).
 template <int EP, int OUT>
-static int launch_i8_pair(I8Args a, cudaStream_t st) {
+static int i8_device_pairs(int& pairs) {
   constexpr int smem = I8PairSmem<EP, OUT>::TOTAL;
   static DeviceOnce attr;
   static int max_pairs_dev[kMaxDevices] = {};  // written under attr's lock, once per device
@@ -957,15 +961,49 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   if (r != B200_OK) return r;
   int dev = 0;
   SDB_CUDA(cudaGetDevice(&dev));
+  pairs = max_pairs_dev[dev];
+  return B200_OK;
+}
+
+// The pair kernel's launch where the device holds `pairs` pairs at once.
+template <int EP, int OUT>
+static b200_launch_plan plan_i8_pair(const I8Args& a, int pairs) {
+  using SM = I8PairSmem<EP, OUT>;
   // Tiles of 192 tokens where the pairs need no more rounds of them: a k-block takes 0.32 us instead of
   // 0.34 and the outputs less (1536 x 2048 x 2048 15.7 -> 14.3 us, 2560 x 2048 x 6144 43.9 -> 41.8); with
   // another round they lose (4096 x 2048 x 2048: 29.2 us against 25.6).
   const int n_tiles = (a.o.n_valid + 255) / 256;
   auto rounds = [&](int bt) {
     const int64_t units = int64_t(n_tiles) * ((a.m + bt - 1) / bt);
-    return (units + max_pairs_dev[dev] - 1) / max_pairs_dev[dev];
+    return (units + pairs - 1) / pairs;
   };
-  a.bt = rounds(192) == rounds(256) ? 192 : 256;
+  const int bt = rounds(192) == rounds(256) ? 192 : 256;
+  // weights beyond what L2 keeps beside the activation stream: groups of about 40 MB
+  const double tile_bytes = 256.0 * a.k;
+  const int groups = n_tiles * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles * tile_bytes / 40e6));
+  b200_launch_plan p = {};
+  p.kernel = B200_KERNEL_INT8_PAIR;
+  p.tile_n = 256;
+  p.tile_m = bt;
+  p.tiles = n_tiles * ((a.m + bt - 1) / bt);
+  p.ctas = 2 * std::min(p.tiles, pairs);
+  p.cluster = 2;
+  p.threads = I8P_THREADS;
+  p.smem_bytes = SM::TOTAL;
+  p.tmem_cols = 512;
+  p.stages = SM::STAGES;
+  p.k_blocks = (a.k + I8_BK - 1) / I8_BK;
+  p.group_tiles = (n_tiles + groups - 1) / groups;
+  return p;
+}
+
+template <int EP, int OUT>
+static int launch_i8_pair(I8Args a, cudaStream_t st) {
+  int pairs = 0;
+  if (int rc = i8_device_pairs<EP, OUT>(pairs)) return rc;
+  const b200_launch_plan p = plan_i8_pair<EP, OUT>(a, pairs);
+  a.bt = p.tile_m;
+  a.ngroup = p.group_tiles;
   CUtensorMap mw, mx, mo;
   constexpr bool SW = EP == B200_EP_SWIGLU;
   if (int rc = SW ? i8_swiglu_map(&mw, a.w, a.o.n_valid / 128, a.k) : i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
@@ -974,19 +1012,71 @@ static int launch_i8_pair(I8Args a, cudaStream_t st) {
   if constexpr (SW && OUT == I8_STAGED) {
     if (int rc = encode_store_tile(&mo, a.o.out, a.m, a.o.n_valid / 2, a.o.ldo, 32, 16)) return rc;
   }
-  const int m_tiles = (a.m + a.bt - 1) / a.bt;
-  // weights beyond what L2 keeps beside the activation stream: groups of about 40 MB
-  const double tile_bytes = 256.0 * a.k;
-  const int groups = n_tiles * tile_bytes <= 48e6 ? 1 : int(std::ceil(n_tiles * tile_bytes / 40e6));
-  a.ngroup = (n_tiles + groups - 1) / groups;
-  const int units = n_tiles * m_tiles;
-  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP, OUT>, dim3(2 * std::min(units, max_pairs_dev[dev])), dim3(I8P_THREADS), smem,
-                      st, mw, mx, mo, a));
+  SDB_CUDA(launch_pdl(gemm_i8_pair_kernel<EP, OUT>, dim3(p.ctas), dim3(I8P_THREADS), p.smem_bytes, st, mw, mx, mo, a));
   return B200_OK;
 }
 
+// How the pair kernel writes these outputs: f(its I8Out).
+template <int EP, typename F>
+static int with_i8_out(const b200_linear_out& o, F f) {
+  constexpr bool SW = EP == B200_EP_SWIGLU;
+  if constexpr (SW) {
+    if (o.lo_offset) return f(std::integral_constant<int, I8_PLANES>{});
+  }
+  if constexpr (EP != B200_EP_STORE) {
+    if (int64_t(o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0 &&
+        (SW || o.n_valid % 4 == 0))
+      return f(std::integral_constant<int, I8_STAGED>{});
+  }
+  return f(std::integral_constant<int, I8_DIRECT>{});
+}
+
+// The split kernel's launch on a device of `sms` SMs.
+static b200_launch_plan plan_i8_split(const I8Args& a, int sms) {
+  const int nk = (a.k + I8_BK - 1) / I8_BK, n_tiles = (a.o.n_valid + 127) / 128;
+  // Tokens of a tile, at most: 128, or with 16 k-blocks or fewer the fewest of 32, 64 and 128 whose
+  // tiles each have an SM. Where K is short, splitting the tokens is cheaper than splitting K, whose
+  // sums cross the cluster (128 x 1024 x 1024 4.6 us against 5.7, 128 x 2048 x 2048 6.6 : 7.3, 96 x
+  // 8224 x 2048 7.6 : 8.3; K 6144, 200 x 2048: 14.4 : 10.2).
+  const bool shallow = nk <= 16;
+  int most = shallow ? 32 : 128;
+  while (most < 128 && int64_t(n_tiles) * ((a.m + most - 1) / most) > sms) most *= 2;
+  int m_tiles = (a.m + most - 1) / most;
+  const int bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
+  m_tiles = (a.m + bt - 1) / bt;
+  const int tiles = n_tiles * m_tiles;
+  // K split over a cluster while SMs would idle and every CTA has two k-blocks. Clusters of 8 only
+  // for at most 32 tokens: they wait longest for their SMs, and each of their CTAs reads as many sums
+  // as one of 4 (2048 x 6144: 32 tokens 7.7 us against 8.3 on clusters of 4, 128 tokens 15.3 : 9.4).
+  // At most 2 with 16 k-blocks or fewer (64 x 2048 x 2048 in tiles of 32: 5.8 us against 6.7 on 4).
+  int split = 1;
+  while (split < (shallow ? 2 : bt <= 32 ? 8 : 4) && 2 * split * tiles <= sms && 4 * split <= nk) split *= 2;
+  // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 300
+  // x 12288 x 2048 17.8 -> 13.2 us), or when that ring holds most of the CTA's K anyway (the next
+  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 12.1 -> 7.7 us), or for clusters of
+  // 8 on most SMs, which else wait for one another's end (32 x 2048 x 8192 13.2 -> 8.7 us; on 64 SMs,
+  // 1024 x 8192, 6.6 : 6.9); else the deeper ring (96 x 12288 x 2048: 8.9 us against 11.7).
+  const int stage = I8S_OP_W + bt * I8_BK, nkb = (nk + split - 1) / split;
+  const bool half = tiles * split > sms || 3 * (I8S_RING_HALF / stage) >= 2 * nkb ||
+                    (split == 8 && 2 * tiles * split > sms);
+  b200_launch_plan p = {};
+  p.kernel = B200_KERNEL_INT8_SPLIT;
+  p.tile_n = 128;
+  p.tile_m = bt;
+  p.tiles = tiles;
+  p.ctas = tiles * split;
+  p.cluster = split;
+  p.threads = 32 * i8s_warps(split);
+  // Two stages at least: the sums take their room.
+  p.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(2, nkb)});
+  p.k_blocks = nkb;
+  p.smem_bytes = i8s_smem(p.stages, bt);
+  p.tmem_cols = i8s_cols(bt);
+  return p;
+}
+
 template <int EP, bool LO, int SPLIT>
-static int launch_i8_cluster(const I8Args& a, int n_tiles, int m_tiles, cudaStream_t st) {
+static int launch_i8_cluster(const I8Args& a, const b200_launch_plan& p, cudaStream_t st) {
   static DeviceOnce attr;
   const int r = once_per_device(attr, [](int) -> int {
     SDB_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<EP, LO, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -997,10 +1087,11 @@ static int launch_i8_cluster(const I8Args& a, int n_tiles, int m_tiles, cudaStre
   CUtensorMap mw, mx;
   if (int rc = i8_map(&mw, a.w, a.n, a.k, a.k, 128)) return rc;
   if (int rc = i8_map(&mx, a.q, a.m, a.k, a.ldx, a.bt)) return rc;
+  const int n_tiles = (a.o.n_valid + 127) / 128;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(SPLIT * n_tiles, m_tiles);
-  cfg.blockDim = dim3(32 * i8s_warps(SPLIT));
-  cfg.dynamicSmemBytes = i8s_smem(a.stages, a.bt);
+  cfg.gridDim = dim3(SPLIT * n_tiles, p.tiles / n_tiles);
+  cfg.blockDim = dim3(p.threads);
+  cfg.dynamicSmemBytes = p.smem_bytes;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1016,39 +1107,14 @@ static int launch_i8_cluster(const I8Args& a, int n_tiles, int m_tiles, cudaStre
 
 template <int EP, bool LO>
 static int launch_i8_split(I8Args a, cudaStream_t st) {
-  const int nk = (a.k + I8_BK - 1) / I8_BK, n_tiles = (a.o.n_valid + 127) / 128;
-  // Tokens of a tile, at most: 128, or with 16 k-blocks or fewer the fewest of 32, 64 and 128 whose
-  // tiles each have an SM. Where K is short, splitting the tokens is cheaper than splitting K, whose
-  // sums cross the cluster (128 x 1024 x 1024 4.6 us against 5.7, 128 x 2048 x 2048 6.6 : 7.3, 96 x
-  // 8224 x 2048 7.6 : 8.3; K 6144, 200 x 2048: 14.4 : 10.2).
-  const bool shallow = nk <= 16;
-  int most = shallow ? 32 : 128;
-  while (most < 128 && int64_t(n_tiles) * ((a.m + most - 1) / most) > sm_count()) most *= 2;
-  int m_tiles = (a.m + most - 1) / most;
-  a.bt = ((a.m + m_tiles - 1) / m_tiles + 15) / 16 * 16;
-  m_tiles = (a.m + a.bt - 1) / a.bt;
-  const int tiles = n_tiles * m_tiles;
-  // K split over a cluster while SMs would idle and every CTA has two k-blocks. Clusters of 8 only
-  // for at most 32 tokens: they wait longest for their SMs, and each of their CTAs reads as many sums
-  // as one of 4 (2048 x 6144: 32 tokens 7.7 us against 8.3 on clusters of 4, 128 tokens 15.3 : 9.4).
-  // At most 2 with 16 k-blocks or fewer (64 x 2048 x 2048 in tiles of 32: 5.8 us against 6.7 on 4).
-  int split = 1;
-  while (split < (shallow ? 2 : a.bt <= 32 ? 8 : 4) && 2 * split * tiles <= sm_count() && 4 * split <= nk) split *= 2;
-  // Half the shared memory per CTA when there are more CTAs than SMs (two run side by side: 300
-  // x 12288 x 2048 17.8 -> 13.2 us), or when that ring holds most of the CTA's K anyway (the next
-  // launch's CTAs then set up beside this one's: 32 x 2048 x 6144 12.1 -> 7.7 us), or for clusters of
-  // 8 on most SMs, which else wait for one another's end (32 x 2048 x 8192 13.2 -> 8.7 us; on 64 SMs,
-  // 1024 x 8192, 6.6 : 6.9); else the deeper ring (96 x 12288 x 2048: 8.9 us against 11.7).
-  const int stage = I8S_OP_W + a.bt * I8_BK, nkb = (nk + split - 1) / split;
-  const bool half = tiles * split > sm_count() || 3 * (I8S_RING_HALF / stage) >= 2 * nkb ||
-                    (split == 8 && 2 * tiles * split > sm_count());
-  // Two stages at least: the sums take their room.
-  a.stages = std::min({I8S_MAX_STAGES, (half ? I8S_RING_HALF : I8S_RING) / stage, std::max(2, nkb)});
-  switch (split) {
-    case 1: return launch_i8_cluster<EP, LO, 1>(a, n_tiles, m_tiles, st);
-    case 2: return launch_i8_cluster<EP, LO, 2>(a, n_tiles, m_tiles, st);
-    case 4: return launch_i8_cluster<EP, LO, 4>(a, n_tiles, m_tiles, st);
-    default: return launch_i8_cluster<EP, LO, 8>(a, n_tiles, m_tiles, st);
+  const b200_launch_plan p = plan_i8_split(a, sm_count());
+  a.bt = p.tile_m;
+  a.stages = p.stages;
+  switch (p.cluster) {
+    case 1: return launch_i8_cluster<EP, LO, 1>(a, p, st);
+    case 2: return launch_i8_cluster<EP, LO, 2>(a, p, st);
+    case 4: return launch_i8_cluster<EP, LO, 4>(a, p, st);
+    default: return launch_i8_cluster<EP, LO, 8>(a, p, st);
   }
 }
 
@@ -1089,19 +1155,17 @@ static int dispatch_i8_reg(const I8Args& a, cudaStream_t st) {
 // 3088 8.6 : 10.1, 32768 x 1024 10.1 : 8.0. With more feature tiles than two a SM, where the split
 // kernel takes more than a round, 1 token 98304 x 2048 30.6 : 36.2, 49152 x 1024 10.0 : 12.5, 49152 x
 // 6144 64 : 57; 16 tokens 98304 x 2048 39.8 : 37.6.
-static bool i8_few_tokens(const I8Args& a, bool swiglu) {
+static bool i8_few_tokens(const I8Args& a, bool swiglu, int sms) {
   if (a.m > I8R_MAX_M) return false;
   const double bytes = double(a.o.n_valid) * a.k;
-  if (a.m <= 8 && a.o.n_valid > 256 * sm_count()) return a.k <= 2048;
+  if (a.m <= 8 && a.o.n_valid > 256 * sms) return a.k <= 2048;
   if (swiglu) return a.m <= 8 ? a.k < 4096 && bytes <= 32e6 : a.k <= 2048 && bytes <= 14e6;
   return a.k < 16384 && bytes <= (a.m <= 8 ? 32e6 : 26e6);
 }
 
-template <int EP>
-static int launch_int8(const I8Args& a, cudaStream_t st) {
-  if (i8_few_tokens(a, EP == B200_EP_SWIGLU)) {
-    return a.m <= 8 ? dispatch_i8_reg<EP, 1>(a, st) : dispatch_i8_reg<EP, 2>(a, st);
-  }
+// The kernel that runs the product on a device of `sms` SMs.
+static b200_linear_kernel i8_kernel(const I8Args& a, bool swiglu, int sms) {
+  if (i8_few_tokens(a, swiglu, sms)) return B200_KERNEL_INT8_REG;
   // Single CTAs while each 128 x 128 tile has an SM (1021 x 2048 x 6144: 17.8 us, pairs 25). With two
   // of them to an SM, pairs if one round of them does (2000 x 2048 x 6144: 27.2 us against 46.2; 300 x
   // 8224 x 2048: 11.7 : 13.1), unless K is short, where two CTAs hide each other's set-up and outputs
@@ -1110,29 +1174,53 @@ static int launch_int8(const I8Args& a, cudaStream_t st) {
   // 18.6 us against 22), but not for 32 tokens or fewer, of which a pair's tile would be almost empty
   // (32 x 98304 x 2048: 37.8 us in single CTAs, several rounds of them, against 43.6; 64 tokens 41 : 43,
   // 100 tokens 46 : 44).
-  const int sms = sm_count();
   const int64_t tiles = int64_t((a.o.n_valid + 127) / 128) * ((a.m + 127) / 128);
   const int64_t pair_tiles = int64_t((a.o.n_valid + 255) / 256) * ((a.m + 255) / 256);
-  constexpr bool SW = EP == B200_EP_SWIGLU;
-  if (tiles <= sms || a.m <= 32 || (tiles <= 2 * sms && (2 * pair_tiles > sms || a.k <= 1024))) {
-    if constexpr (SW) {
-      if (a.o.lo_offset) return launch_i8_split<EP, true>(a, st);
-    }
-    return launch_i8_split<EP, false>(a, st);
-  }
-  if constexpr (SW) {
-    if (a.o.lo_offset) return launch_i8_pair<EP, I8_PLANES>(a, st);
-  }
-  if constexpr (EP != B200_EP_STORE) {
-    if (int64_t(a.o.ldo) * (SW ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.o.out) & 15) == 0 &&
-        (SW || a.o.n_valid % 4 == 0))
-      return launch_i8_pair<EP, I8_STAGED>(a, st);
-  }
-  return launch_i8_pair<EP, I8_DIRECT>(a, st);
+  return tiles <= sms || a.m <= 32 || (tiles <= 2 * sms && (2 * pair_tiles > sms || a.k <= 1024))
+             ? B200_KERNEL_INT8_SPLIT
+             : B200_KERNEL_INT8_PAIR;
 }
 
-int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
-                    const b200_linear_out* out, cudaStream_t st) {
+template <int EP>
+static int launch_int8(const I8Args& a, cudaStream_t st) {
+  constexpr bool SW = EP == B200_EP_SWIGLU;
+  switch (i8_kernel(a, SW, sm_count())) {
+    case B200_KERNEL_INT8_REG: return a.m <= 8 ? dispatch_i8_reg<EP, 1>(a, st) : dispatch_i8_reg<EP, 2>(a, st);
+    case B200_KERNEL_INT8_SPLIT:
+      if constexpr (SW) {
+        if (a.o.lo_offset) return launch_i8_split<EP, true>(a, st);
+      }
+      return launch_i8_split<EP, false>(a, st);
+    default: return with_i8_out<EP>(a.o, [&](auto out) { return launch_i8_pair<EP, decltype(out)::value>(a, st); });
+  }
+}
+
+// launch_int8's choices on a device of `sms` SMs (0: the current one).
+template <int EP>
+static int plan_int8(const I8Args& a, int sms, b200_launch_plan& p) {
+  const int n_sm = sms ? sms : sm_count();
+  p = {};
+  switch (i8_kernel(a, EP == B200_EP_SWIGLU, n_sm)) {
+    case B200_KERNEL_INT8_REG:
+      p.kernel = B200_KERNEL_INT8_REG;
+      p.cluster = 1;
+      return B200_OK;
+    case B200_KERNEL_INT8_SPLIT: p = plan_i8_split(a, n_sm); return B200_OK;
+    default:
+      return with_i8_out<EP>(a.o, [&](auto out) -> int {
+        int pairs = std::max(1, sms / 2);
+        if (!sms) {
+          if (int rc = i8_device_pairs<EP, decltype(out)::value>(pairs)) return rc;
+        }
+        p = plan_i8_pair<EP, decltype(out)::value>(a, pairs);
+        return B200_OK;
+      });
+  }
+}
+
+// The arguments of b200_linear_int8, checked.
+static int i8_args(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
+                   const b200_linear_out* out, I8Args& a) {
   if (!q || !x_scale || !w || !out || !w->data || !out->out)
     return sdb_fail(B200_ERR_ARG, "b200_linear_int8: null pointer");
   if (w->format != B200_W_INT8) return sdb_fail(B200_ERR_FORMAT, "b200_linear_int8: needs a B200_W_INT8 weight");
@@ -1158,8 +1246,15 @@ int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k,
     return sdb_fail(B200_ERR_ARG, "b200_linear_int8: unknown lo_format");
   if ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w->row_scale)) & 3)
     return sdb_fail(B200_ERR_SHAPE, "b200_linear_int8: scales are not aligned to their elements");
-  I8Args a{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx, 1, 0, 0, 0};
+  a = I8Args{q, x_scale, static_cast<const int8_t*>(w->data), w->row_scale, *out, m, w->n, k, ldx, 1, 0, 0, 0};
   a.vec = out->ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out->out) & (swiglu ? 7 : 15)) == 0;
+  return B200_OK;
+}
+
+int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx, const b200_qweight* w,
+                    const b200_linear_out* out, cudaStream_t st) {
+  I8Args a;
+  if (int rc = i8_args(q, x_scale, m, k, ldx, w, out, a)) return rc;
   switch (out->epilogue) {
     case B200_EP_STORE: return launch_int8<B200_EP_STORE>(a, st);
     case B200_EP_RESID_ADD: return launch_int8<B200_EP_RESID_ADD>(a, st);
@@ -1172,4 +1267,18 @@ int sdb_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k,
 extern "C" int b200_linear_int8(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx,
                                 const b200_qweight* w, const b200_linear_out* out, b200_stream stream) {
   return sdb::sdb_linear_int8(q, x_scale, m, k, ldx, w, out, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200_linear_int8_plan(const int8_t* q, const float* x_scale, int32_t m, int32_t k, int32_t ldx,
+                                     const b200_qweight* w, const b200_linear_out* out, int32_t sms,
+                                     b200_launch_plan* plan) {
+  using namespace sdb;
+  if (!plan || sms < 0) return sdb_fail(B200_ERR_ARG, "b200_linear_int8_plan: no plan, or a negative number of SMs");
+  I8Args a;
+  if (int rc = i8_args(q, x_scale, m, k, ldx, w, out, a)) return rc;
+  switch (out->epilogue) {
+    case B200_EP_STORE: return plan_int8<B200_EP_STORE>(a, sms, *plan);
+    case B200_EP_RESID_ADD: return plan_int8<B200_EP_RESID_ADD>(a, sms, *plan);
+    default: return plan_int8<B200_EP_SWIGLU>(a, sms, *plan);
+  }
 }
