@@ -74,3 +74,24 @@ def test_plans_refuse_what_the_linears_refuse():
     assert P.bf16_plan(64, 256, 128).kernel == _lib.KERNEL_OTHER
     assert P.int8_plan(1, 2048, 2048).kernel == _lib.KERNEL_INT8_REG
     assert P.int8_plan(8192, 2048, 2048, sms=1).ctas == 2
+
+
+def _turns(p):
+    """How often the k-blocks pass the ring."""
+    return p.k_blocks / p.stages
+
+
+def test_the_ring_cases_pass_rings_of_every_depth():
+    for m, n, k, ep, cluster, stages in P.RINGS:
+        p = P.int8_plan(m, n, k, ep)
+        assert (p.kernel, p.cluster, p.stages) == (_lib.KERNEL_INT8_SPLIT, cluster, stages), (m, n, k)
+        assert _turns(p) > 1, (m, n, k)
+    assert {c[5] for c in P.RINGS} == set(range(3, 13))
+    # a barrier serves every second turn: at every depth some are used again
+    assert {c[5] for c in P.RINGS if _turns(P.int8_plan(*c[:4])) > 2} == set(range(3, 13))
+    p = P.int8_plan(*P.RINGS[0][:4])
+    assert p.ctas > 148 and p.k_blocks == 16 and p.smem_bytes + 1024 <= 114 * 1024
+    for m, n, k in itertools.product(TOKENS, OUTPUTS, DEPTHS):   # what the list leaves out is not reached
+        p = P.int8_plan(m, n, k)
+        if p.kernel == _lib.KERNEL_INT8_SPLIT:
+            assert p.stages >= 3 or p.k_blocks <= p.stages
