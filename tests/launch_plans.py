@@ -42,3 +42,7 @@ RINGS = [(300, 12288, 2048, "swiglu", 1, 3), (300, 12288, 1040, "store", 1, 3), 
          (17, 128, 65536, "swiglu", 8, 11),
          (1, 12288, 3088, "store", 1, 12), (8, 6144, 8208, "residual", 2, 12), (16, 4096, 16384, "swiglu", 4, 12),
          (8, 1000, 65536, "store", 8, 12)]
+
+# (m, n, k, tokens per tile): products of the int8 pair kernel whose weights are taken in several
+# groups of output tiles, the last of them smaller, with more tiles than pairs
+GROUPS = [(600, 12032, 8192, 256), (760, 6400, 16384, 192)]

@@ -67,3 +67,30 @@ def test_operand_rings_passed_several_times(m, n, k, ep, cluster, stages):
     _check(outs[0], base, ref, ep)
     for out in outs[1:]:
         assert torch.equal(out, outs[0])
+
+
+@pytest.mark.parametrize("m,n,k,tokens", P.GROUPS)
+@pytest.mark.parametrize("ep,form", [("store", ""), ("residual", ""), ("residual", "unaligned"), ("swiglu", ""),
+                                     ("swiglu", "unaligned"), ("swiglu", "low plane")])
+def test_weights_in_several_groups(m, n, k, tokens, ep, form):
+    """Each output tile once, in groups that are not all of one size, in every way of writing it."""
+    from strands_decider_b200 import _lib, int8
+
+    q, s, w, base, ref = _case(m, n, k, ep)
+    cols = base.shape[1]
+    wide = torch.full((m, cols + 9), 5.0, dtype=base.dtype, device="cuda")
+    out = wide[:, 1:1 + cols].copy_(base) if form == "unaligned" else base.clone()
+    lo = torch.zeros_like(base) if form == "low plane" else None
+    p = P.int8_plan(m, n, k, ep, lo=64 if lo is not None else 0, sms=0, ldo=out.stride(0), out=out.data_ptr())
+    tiles = -(-n // 256)
+    assert p.kernel == _lib.KERNEL_INT8_PAIR and p.tile_m == tokens
+    assert p.group_tiles < tiles and tiles % p.group_tiles and 2 * p.tiles > p.ctas
+    int8.linear(q, s, w, out, epilogue=ep, lo=lo)
+    _check(out, base, ref, ep)
+    if lo is not None:
+        y = ref.reshape(m, -1, 2, 64)
+        h = (y[:, :, 0] * torch.sigmoid(y[:, :, 0]) * y[:, :, 1]).reshape(out.shape)
+        fast = 2.0 ** -17 + y[:, :, 0].abs().max().item() * 2.0 ** -22
+        assert ((out.double() + lo.double() - h).abs() <= (2.0 ** -16 + 2 * fast) * h.abs()).all()
+    if form == "unaligned":
+        assert (wide[:, :1] == 5).all() and (wide[:, 1 + cols:] == 5).all()

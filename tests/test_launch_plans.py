@@ -95,3 +95,12 @@ def test_the_ring_cases_pass_rings_of_every_depth():
         p = P.int8_plan(m, n, k)
         if p.kernel == _lib.KERNEL_INT8_SPLIT:
             assert p.stages >= 3 or p.k_blocks <= p.stages
+
+
+def test_the_group_cases_have_several_uneven_groups():
+    for m, n, k, tokens in P.GROUPS:
+        for ep in ("store", "residual", "swiglu"):
+            p = P.int8_plan(m, n, k, ep)
+            tiles_n = -(-n // 256)
+            assert p.kernel == _lib.KERNEL_INT8_PAIR and p.tile_m == tokens
+            assert p.group_tiles < tiles_n and tiles_n % p.group_tiles and p.tiles > 74
