@@ -8,6 +8,8 @@ non-zero status. Tensors are passed as raw device pointers (torch owns the memor
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -192,11 +194,14 @@ def int8_ops():
     global _int8_ops
     if _int8_ops is None:
         lib = load()
-        try:
-            from . import _int8_ops as ops
-        except ImportError as e:
-            raise RuntimeError(f"{_build.OPS} does not load ({e}): build it with `python -m strands_decider_b200.build`") \
-                from e
+        path = _build.ops_path()
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing (it belongs to one torch and one Python): build it with "
+                               "`python -m strands_decider_b200.build`")
+        name = __package__ + "._int8_ops"
+        spec = importlib.util.spec_from_loader(name, importlib.machinery.ExtensionFileLoader(name, path))
+        ops = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ops)
         ops.bind(*(C.cast(getattr(lib, name), C.c_void_p).value
                    for name in ("b200_quantize_act_int8", "b200_rmsnorm_int8", "b200_linear_int8")))
         _int8_ops = ops

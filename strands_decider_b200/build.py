@@ -6,13 +6,17 @@ Each .cu in csrc/ is compiled for sm_100a only (`-gencode arch=compute_100a,code
 as relocatable device code, then device-linked into one shared library. Rebuilds only
 when a source or header is newer than the library (or with --force).
 
-csrc/int8_torch.cpp becomes the Python extension module _int8_ops.so beside this file: host code
-over torch's headers, which takes the library's entry points by address and links nothing of it.
+csrc/int8_torch.cpp becomes the Python extension module _int8_ops, in the same folder: host code over
+torch's headers, which takes the library's entry points by address and links nothing of it. It is
+compiled against one torch and one Python, so its file is named after both: after a change of either
+it is missing, not loaded against other layouts. Processes that build at once take turns.
 """
 
 from __future__ import annotations
 
 import argparse
+import contextlib
+import fcntl
 import glob
 import os
 import shutil
@@ -29,7 +33,6 @@ LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libstrands_b200.so")
 OBJDIR = os.path.join(PKG, "_build")
 OPS_SRC = os.path.join(CSRC, "int8_torch.cpp")
-OPS = os.path.join(PKG, "_int8_ops.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
@@ -58,15 +61,37 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in _inputs())
 
 
-def build_ops(force: bool = False) -> str:
-    """The extension module of the int8 operators' Python calls."""
+@contextlib.contextmanager
+def _turn():
+    """One build at a time in this tree."""
+    os.makedirs(LIBDIR, exist_ok=True)
+    os.makedirs(OBJDIR, exist_ok=True)
+    with open(os.path.join(OBJDIR, "lock"), "w") as f:
+        fcntl.flock(f, fcntl.LOCK_EX)
+        yield
+
+
+def ops_path() -> str:
+    """The extension module of the int8 operators' Python calls, for the running torch and Python."""
+    import torch
+
+    abi = "" if torch.compiled_with_cxx11_abi() else "-precxx11"
+    return os.path.join(LIBDIR, f"_int8_ops-torch{torch.__version__}-{(torch.version.git_version or '')[:10]}{abi}"
+                                f"{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
+def ops_up_to_date() -> bool:
+    ops = ops_path()
     inputs = [OPS_SRC, os.path.join(INCLUDE, "strands_b200.h"), __file__]
-    if not force and os.path.exists(OPS) and all(os.path.getmtime(p) <= os.path.getmtime(OPS) for p in inputs):
-        return OPS
+    return os.path.exists(ops) and all(os.path.getmtime(p) <= os.path.getmtime(ops) for p in inputs)
+
+
+def _compile_ops() -> None:
     import torch
 
     root = os.path.dirname(torch.__file__)
-    tmp = OPS + ".tmp"
+    ops = ops_path()
+    tmp = f"{ops}.{os.getpid()}.tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}",
            "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(root, "include"),
@@ -75,18 +100,29 @@ def build_ops(force: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on {os.path.basename(OPS_SRC)}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, OPS)
-    return OPS
+    os.replace(tmp, ops)
+
+
+def build_ops(force: bool = False) -> str:
+    """Build the extension module where it is missing or older than its sources."""
+    if force or not ops_up_to_date():
+        with _turn():
+            if force or not ops_up_to_date():   # another process may have built it meanwhile
+                _compile_ops()
+    return ops_path()
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False, extra: list[str] | None = None) -> str:
     build_ops(force)
-    if not force and up_to_date():
-        return LIB
-    os.makedirs(LIBDIR, exist_ok=True)
-    os.makedirs(OBJDIR, exist_ok=True)
+    if force or not up_to_date():
+        with _turn():
+            if force or not up_to_date():
+                _compile_library(jobs, verbose, extra or [])
+    return LIB
+
+
+def _compile_library(jobs: int | None, verbose: bool, extra: list[str]) -> None:
     cc = nvcc()
-    extra = extra or []
 
     def compile_one(src: str) -> str:
         obj = os.path.join(OBJDIR, os.path.basename(src)[:-3] + ".o")
@@ -100,13 +136,12 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, e
 
     with ThreadPoolExecutor(max_workers=jobs or os.cpu_count() or 4) as ex:
         objs = list(ex.map(compile_one, sources()))
-    tmp = LIB + ".tmp"
+    tmp = f"{LIB}.{os.getpid()}.tmp"
     cmd = [cc, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", tmp, *objs, "-lcudart_static", "-ldl", "-lrt", "-lpthread"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    return LIB
 
 
 def main() -> None:
