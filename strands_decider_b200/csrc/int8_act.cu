@@ -287,57 +287,44 @@ __global__ void __launch_bounds__(row_threads<TPR>()) quantize_int8_kernel(const
 struct RowShape {
   int tpr, nv;
 };
+constexpr int next_nv(int nv) { return nv == 3 ? 4 : nv == 6 ? 8 : nv == 12 ? 16 : nv + (nv + 1) / 2; }
 static RowShape row_shape(int rows, int units, int cap) {
   int tpr = units <= 32 ? 8 : 32;
   while (tpr < 512 && (units > cap * tpr || (int64_t(rows) * tpr < 512 * int64_t(sm_count()) && units > tpr))) tpr *= 4;
   if (units > 16 * tpr) tpr = 1024;
   int nv = 1;
-  while (nv * tpr < units) nv = nv == 3 ? 4 : nv == 6 ? 8 : nv == 12 ? 16 : nv + (nv + 1) / 2;
+  while (nv * tpr < units) nv = next_nv(nv);
   return {tpr, nv};
 }
+template <bool NORM, int KIND>
+constexpr int row_cap() { return NORM ? (KIND == ACT_NONE ? 16 : 8) : (KIND == ACT_PLANES ? 4 : 16); }
 
-template <int KIND, int TPR, int NV, bool NORM>
-static int launch_row_kernel(const RowArgs& a, cudaStream_t st) {
-  constexpr int rpb = rows_per_block<TPR>();
-  const dim3 grid((a.rows + rpb - 1) / rpb), block(row_threads<TPR>());
-  if constexpr (NORM) SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<TPR, NV, KIND>, grid, block, 0, st, a));
-  else SDB_CUDA(launch_pdl(quantize_int8_kernel<TPR, NV, KIND>, grid, block, 0, st, a));
-  return B200_OK;
-}
-template <bool NORM, int KIND, int TPR>
+template <bool NORM, int KIND, int TPR, int NV>
 static int launch_nv(const RowArgs& a, int nv, cudaStream_t st) {
-  if constexpr (TPR == 1024) {  // only rows that no block of 512 holds
-    return launch_row_kernel<KIND, TPR, 16, NORM>(a, st);
-  } else {
-    switch (nv) {
-      case 1: return launch_row_kernel<KIND, TPR, 1, NORM>(a, st);
-      case 2: return launch_row_kernel<KIND, TPR, 2, NORM>(a, st);
-      case 3: return launch_row_kernel<KIND, TPR, 3, NORM>(a, st);
-      case 4: return launch_row_kernel<KIND, TPR, 4, NORM>(a, st);
-      default: break;
-    }
-    if constexpr (TPR > 8) {
-      switch (nv) {
-        case 6: return launch_row_kernel<KIND, TPR, 6, NORM>(a, st);
-        case 8: return launch_row_kernel<KIND, TPR, 8, NORM>(a, st);
-        case 12: return launch_row_kernel<KIND, TPR, 12, NORM>(a, st);
-        case 16: return launch_row_kernel<KIND, TPR, 16, NORM>(a, st);
-        default: break;
-      }
-    }
-    return sdb_fail(B200_ERR_SHAPE, "int8 rows: no such shape");  // 8 lanes hold at most 32 groups
+  if (nv == NV) {
+    constexpr int rpb = rows_per_block<TPR>();
+    const dim3 grid((a.rows + rpb - 1) / rpb), block(row_threads<TPR>());
+    if constexpr (NORM) SDB_CUDA(launch_pdl(rmsnorm_int8_kernel<TPR, NV, KIND>, grid, block, 0, st, a));
+    else SDB_CUDA(launch_pdl(quantize_int8_kernel<TPR, NV, KIND>, grid, block, 0, st, a));
+    return B200_OK;
   }
+  // groups that row_shape gives a thread: 8 lanes hold at most 32, 32 and 128 threads the cap each
+  constexpr int most = TPR == 8 ? 4 : TPR >= 512 ? 16 : row_cap<NORM, KIND>();
+  if constexpr (next_nv(NV) <= most) return launch_nv<NORM, KIND, TPR, next_nv(NV)>(a, nv, st);
+  else return sdb_fail(B200_ERR_SHAPE, "int8 rows: no such shape");
 }
 template <bool NORM, int KIND>
 static int launch_rows(const RowArgs& a, cudaStream_t st) {
-  constexpr int cap = NORM ? (KIND == ACT_NONE ? 16 : 8) : (KIND == ACT_PLANES ? 4 : 16);
-  const RowShape r = row_shape(a.rows, a.k / (NORM || KIND == B200_ACT_F32 ? 4 : 8), cap);
+  constexpr int E = NORM || KIND == B200_ACT_F32 ? 4 : 8;
+  const RowShape r = row_shape(a.rows, a.k / E, row_cap<NORM, KIND>());
   switch (r.tpr) {
-    case 8: return launch_nv<NORM, KIND, 8>(a, r.nv, st);
-    case 32: return launch_nv<NORM, KIND, 32>(a, r.nv, st);
-    case 128: return launch_nv<NORM, KIND, 128>(a, r.nv, st);
-    case 512: return launch_nv<NORM, KIND, 512>(a, r.nv, st);
-    default: return launch_nv<NORM, KIND, 1024>(a, r.nv, st);
+    case 8: return launch_nv<NORM, KIND, 8, 1>(a, r.nv, st);
+    case 32: return launch_nv<NORM, KIND, 32, 1>(a, r.nv, st);
+    case 128: return launch_nv<NORM, KIND, 128, 1>(a, r.nv, st);
+    case 512: return launch_nv<NORM, KIND, 512, 1>(a, r.nv, st);
+    default:  // rows that no block of 512 holds
+      if constexpr (I8_K_MAX / E > 16 * 512) return launch_nv<NORM, KIND, 1024, 16>(a, 16, st);
+      else return sdb_fail(B200_ERR_SHAPE, "int8 rows: no such shape");
   }
 }
 
