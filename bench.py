@@ -210,11 +210,7 @@ def launches_per_forward(spec: config.ModelSpec, decide: bool, tokens: int = 0, 
     mixer's 2 kernels, plus a zeroing kernel before a split-K in-projection (batches of 129 to
     4095 tokens; up to 128 tokens on packed weights the norm before it clears the output);
     forwards of >= 4096 tokens also dequantise each of the 4 weights per layer once (bf16
-    weights too with the e4m3 low plane); the slot-length update when states are saved; the head.
-    Int8 weights (W8A8): per layer 2 norms, 4 GEMMs, the mixer's 2 kernels and 2 activation
-    quantisers at every size."""
-    if spec.weight_format == "int8":
-        return 1 + (1 if decide else 0) + (1 if saves else 0) + 10 * len(spec.layer_types)
+    weights too with the e4m3 low plane); the slot-length update when states are saved; the head."""
     big = tokens >= 4096
     folded = tokens <= 128 and spec.weight_format != "bf16"
     dq = 4 if big and (spec.weight_format != "bf16" or lo_plane == "e4m3") else 0
@@ -613,10 +609,66 @@ def small_kernels_case(tokens: int = 8192, rows: int = 384):
     return launch, None
 
 
+def forward_case(fmt: str, requests: int = 128, length: int = 512) -> list[tuple[str, float]]:
+    """(what, median ms) of three forwards of the 2B shape with weights in `fmt`, each a CUDA graph
+    replayed alone: states of `length` tokens into their slots, one 96-token request with its decision,
+    and one token appended to each of 8 states."""
+    from strands_decider_b200.runtime import DecisionModel
+
+    spec = config.HYBRID_2B.with_format(fmt)
+    reps, room = 20, 64
+    m = DecisionModel(WT.DeviceWeights.synthetic(spec, seed=0), max_tokens=requests * length, pool_slots=requests,
+                      pool_kv_tokens=requests * (length + room))
+    ids = torch.randint(0, spec.vocab, (requests * length,), generator=torch.Generator().manual_seed(0))
+
+    def dev(x):
+        return torch.as_tensor(x, dtype=torch.int32).cuda()
+
+    ids, slots = dev(ids), dev(range(requests))
+    m.slot_kv.copy_(dev([i * (length + room) for i in range(requests)]))
+    decide = {"last_tok": dev([95]), "opt_ids": dev([[11, 12, 13]]), "n_opts": dev([3]), "kinds": dev([1]),
+              "temps": torch.ones(1, device="cuda")}
+    cu = dev(range(0, requests * length + 1, length))
+    few = min(8, requests)
+    one, cu1, cu8, own = ids[:96].contiguous(), dev([0, 96]), dev(range(few + 1)), slots[:few].contiguous()
+    tok = ids[:few].contiguous()
+    out = []
+    for what, launch in ((f"{requests} states of {length} tokens", lambda st: m.forward(ids, cu, None, slots, None, length, st)),
+                         ("one 96-token request", lambda st: m.forward(one, cu1, None, None, decide, 96, st)),
+                         (f"one token appended to {few} states", lambda st: m.forward(tok, cu8, own, own, None, 1, st))):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            launch(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            launch(side)
+        for _ in range(3):
+            graph.replay()
+        times = []
+        for _ in range(reps):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            graph.replay()
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        out.append((what, statistics.median(times)))
+    if _lib.read_fault():
+        raise RuntimeError("a kernel recorded a fault")
+    return out
+
+
 def run_case(args) -> None:
     if not torch.cuda.is_available():
         raise SystemExit("--case needs a CUDA device")
     _lib.load()
+    if args.case == "forward":
+        for what, ms in forward_case(args.fmt):
+            print(f"{args.fmt}, {what}: {ms:.3f} ms", flush=True)
+        return
     if args.case == "small":
         launch, flops = small_kernels_case()
         label = "embed, rmsnorm (bf16 / e4m3 low plane), decide, pointer readout, dequantise, quantise (2B shapes)"
@@ -998,8 +1050,9 @@ def main() -> None:
                          "single-request latency to the line")
     ap.add_argument("--lo-plane", default="e4m3", choices=["bf16", "e4m3"],
                     help="low activation plane of the large-batch GEMMs (DecisionModel lo_plane)")
-    ap.add_argument("--case", choices=["gemm", "gdn", "attention", "small"],
-                    help="time (and profile) one kernel alone (small: the head, norm, embedding and (de)quantisers)")
+    ap.add_argument("--case", choices=["gemm", "gdn", "attention", "small", "forward"],
+                    help="time (and profile) one kernel alone (small: the head, norm, embedding and (de)quantisers); "
+                         "forward: time three forwards of the 2B shape with weights in --fmt")
     ap.add_argument("--m", type=int, default=8192)
     ap.add_argument("--fmt", default="nvfp4", choices=list(config.WEIGHT_FORMATS))
     ap.add_argument("--ep", default="swiglu", choices=["swiglu", "store", "resid"])
