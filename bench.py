@@ -611,7 +611,7 @@ def small_kernels_case(tokens: int = 8192, rows: int = 384):
 
 def forward_case(fmt: str, requests: int = 128, length: int = 512) -> list[tuple[str, float]]:
     """(what, median ms) of three forwards of the 2B shape with weights in `fmt`, each a CUDA graph
-    replayed alone: states of `length` tokens into their slots, one 96-token request with its decision,
+    whose replays follow one another: states of `length` tokens into their slots, one 96-token request with its decision,
     and one token appended to each of 8 states."""
     from strands_decider_b200.runtime import DecisionModel
 
@@ -646,15 +646,13 @@ def forward_case(fmt: str, requests: int = 128, length: int = 512) -> list[tuple
             launch(side)
         for _ in range(3):
             graph.replay()
-        times = []
-        for _ in range(reps):
-            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-            torch.cuda.synchronize()
-            a.record()
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(reps + 1)]
+        ev[0].record()
+        for e in ev[1:]:
             graph.replay()
-            b.record()
-            b.synchronize()
-            times.append(a.elapsed_time(b))
+            e.record()
+        torch.cuda.synchronize()
+        times = [a.elapsed_time(b) for a, b in zip(ev, ev[1:])]
         out.append((what, statistics.median(times)))
     if _lib.read_fault():
         raise RuntimeError("a kernel recorded a fault")
