@@ -443,7 +443,8 @@ typedef struct b200_model_config {
   float eps;
   /* The format of every layer weight. B200_W_INT8: the forward runs W8A8, every linear on
    * b200_linear_int8 and its input as the int8 codes of b200_rmsnorm_int8 / b200_quantize_act_int8
-   * (no activation planes: dequant_min_tokens and lo_format are not used); needs eps > 0. */
+   * (no activation planes: dequant_min_tokens and lo_format are not used); needs eps > 0 and no
+   * linear of more than 65536 input features. */
   int32_t weight_format;
   /* Batches of at least this many tokens dequantise each packed weight once per GEMM into a
    * bf16 [N, K] workspace buffer and run the GEMM on it (the in-kernel unpack would repeat for

@@ -302,6 +302,10 @@ extern "C" int b200_model_create(const b200_model_config* cfg, b200_model** out)
     delete m;
     return sdb_fail(B200_ERR_UNSUPPORTED, "b200_model_create: GDN layers need dk = dv = 128, conv width 4");
   }
+  if (m->int8() && std::max({cfg->hidden, cfg->inter, ng ? m->value_dim() : 0, na ? m->attn_o_in() : 0}) > 65536) {
+    delete m;
+    return sdb_fail(B200_ERR_SHAPE, "b200_model_create: int8 linears take at most 65536 input features");
+  }
   *out = m;
   return B200_OK;
 }
