@@ -182,9 +182,11 @@ int b200_linear_nvfp4_native(const uint8_t* x_codes, const uint8_t* x_sf, int32_
 /* ---------------------------------------------------------------- 8-bit integer linears (W8A8)
  * Activations and weights as int8 codes with one fp32 scale per token and one per output channel:
  *   y[t, n] = (sum_k q[t, k] * w[n, k]) * scale[t] * row_scale[n],
- * the sum exact in int32. Replaces the same `nn.Linear` calls as b200_linear (TF:417-420,
- * TF:632-643, TF:701-703) at twice the bf16 tensor rate and in one pass, at about 7 significant
- * bits per activation row: for callers that accept W8A8 (a model of B200_W_INT8 weights runs on
+ * the sum exact in int32, times scale[t] (this product must stay below 2^128: any scale[t] up to
+ * 2^97 does), times row_scale[n], each one fp32 rounding. Replaces the same `nn.Linear` calls as
+ * b200_linear (TF:417-420, TF:632-643, TF:701-703) at twice the bf16 tensor rate and in one pass,
+ * at about 7 significant bits per activation row: for callers that accept W8A8 (a model of
+ * B200_W_INT8 weights runs on
  * it, see b200_model_create).
  *
  * Codes of a row v[0..k) (fp32; fl = one fp32 rounding, rint = half to even):

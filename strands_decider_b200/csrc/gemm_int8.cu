@@ -10,7 +10,9 @@
 //   gemm_i8_pair_kernel   CTA pairs, 256 features x 256 or 192 tokens, persistent (large products)
 //   gemm_i8_split_kernel  one CTA per 128 features x up to 128 tokens and K range; the K ranges of
 //                         a tile are a cluster that adds its sums through distributed shared memory
-//   gemm_i8_reg_kernel    at most 16 tokens and weights of some MB: these through registers into mma.sync
+//   gemm_i8_reg_kernel    at most 16 tokens: weights through registers into mma.sync, up to 32 MB of
+//                         them (26 from 9 tokens on, fewer for the SwiGLU), or for at most 8 tokens and
+//                         K <= 2048 as many as there are once the outputs pass 256 a SM (i8_few_tokens)
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

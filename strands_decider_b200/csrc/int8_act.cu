@@ -10,9 +10,10 @@
 //
 // Every row is read once: its elements stay in the registers of the threads that share it while
 // the sum, the maximum and the codes follow one another. Bound by HBM where there are rows enough:
-// norm 65536 x 2048 108 us = 6.2 TB/s (then by the instructions of a row), 12288 x 2048
-// with an fp32 delta 50.7 us = 6.5 TB/s; codes of 65536 x 6144 bf16 173 us = 7.0 TB/s, of 12288 x
-// 2048 two planes 19.6 us = 5.7 TB/s; one row of 2048 is a chain of latencies, 2.2 and 1.6 us.
+// norm 65536 x 2048 108 us = 6.2 TB/s (117 us a launch in a run of 5000), 12288 x 2048
+// with an fp32 delta 50.7 us = 6.5 TB/s; codes of 65536 x 6144 bf16 174 us = 6.9 TB/s, of 12288 x
+// 2048 two planes 19.4 us = 6.5 TB/s; one row is a chain of latencies, 2.0 us of norm (2048), 1.5 of
+// codes (6144).
 #include "common.cuh"
 
 namespace sdb {
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(row_threads<TPR>()) rmsnorm_int8_kernel(const 
   const float4* wr = reinterpret_cast<const float4*>(a.w);
   // A warp's weights in batches, whose loads are in flight together (3844 x 784 9.0 -> 6.4 us, 20000 x
   // 1392 39.7 -> 32.6). Not of its longest rows, whose registers they would take (65536 x 2048: 202 us
-  // against 116), and not in blocks of a row, of which enough are resident (28162 x 2512 73 : 68).
+  // against 116 at the time), and not in blocks of a row, of which enough are resident (28162 x 2512 73 : 68).
   constexpr int B = TPR > 32 || NV > 12 ? 1 : NV % 4 == 0 ? 4 : NV % 3 == 0 ? 3 : NV;
 #pragma unroll
   for (int i0 = 0; i0 < NV; i0 += B) {
@@ -279,7 +280,8 @@ __global__ void __launch_bounds__(row_threads<TPR>()) quantize_int8_kernel(const
 // hold the row in `cap` groups each: a warp's reductions need no barrier and all of its loads are
 // in flight at once, but a row that comes in two arrays fills the registers sooner (planes at 12288
 // x 2048: 19.5 us with 128 threads a row, 22.1 with 32; an fp32 delta at 12288 x 2048: 50.6 against
-// 59.2; no delta at 65536 x 2048: 116 us with 32, 123 with 128). Four times as many while the
+// 59.2; no delta at 65536 x 2048: 116 us with 32, 123 with 128, both before codes were rounded by an
+// addition; 108 since). Four times as many while the
 // device has under 512 threads per SM and the row has work for them (1 x 2048: 2.1 us against 2.5).
 // Rows of at most 32 groups take 8 lanes, four rows to a warp. A thread's groups are 1, 2, 3, 4, 6, 8,
 // 12 or 16: registers for twice as many as the row has would leave fewer rows in flight (codes of
