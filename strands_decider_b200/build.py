@@ -19,6 +19,7 @@ import contextlib
 import fcntl
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -76,8 +77,8 @@ def ops_path() -> str:
     import torch
 
     abi = "" if torch.compiled_with_cxx11_abi() else "-precxx11"
-    return os.path.join(LIBDIR, f"_int8_ops-torch{torch.__version__}-{(torch.version.git_version or '')[:10]}{abi}"
-                                f"{sysconfig.get_config_var('EXT_SUFFIX')}")
+    version = re.sub(r"[^\w.]", "_", f"{torch.__version__}-{(torch.version.git_version or '')[:10]}")
+    return os.path.join(LIBDIR, f"_int8_ops-torch{version}{abi}{sysconfig.get_config_var('EXT_SUFFIX')}")
 
 
 def ops_up_to_date() -> bool:
